@@ -434,6 +434,113 @@ int muse_encode12_device_escapes(const void* w, int64_t n, int64_t k, const uint
 int muse_decode12(const uint8_t* planes, const uint8_t* bases, const int32_t* esc_ptr, const uint32_t* esc_val,
                   int64_t n, int64_t k, uint16_t* w_out, int threads);
 
+/* ---- between the projections: rotary positions and the paged cache, attention over it, expert routing ----
+ *
+ * The reference has no counterpart of these (it times the projections alone, reference.py:1-8); they are the
+ * operators a decode, verify or prompt step runs between its qkv_gate and o projections (16 query heads and
+ * 2 key/value heads of 64 plus a 16 x 64 gate on each GPU) and after its router. Strides are in elements, the
+ * last dimension of every tensor is contiguous. All pointers are device pointers; launches use programmatic
+ * dependent launch and read no input before the previous grid in the stream has completed, but for constants
+ * named at each.
+ */
+
+/* 16-bit types of q, k, v, the cache, the gate and the output. */
+#define MUSE_BF16 0
+#define MUSE_F16 1
+#define MUSE_F32 2 /* muse_route's logits only */
+
+/*
+ * Rotary positions on q and k, and k, v appended to a paged cache, in one launch. For each rotated pair (x, y)
+ * of a head at position p, with the table's cosine c and sine s: (x c - y s, y c + x s) in FP32, rounded once.
+ * Pair i is entries (2i, 2i + 1) when `interleaved`, else (i, i + rotary / 2); entries past `rotary` are copied.
+ * k and v of token t go to page slot / page_size, entry slot % page_size; a negative slot appends nothing (the
+ * row's q is still written). Slots of one call are distinct. q_out may be q. A position outside
+ * [0, positions) or a slot outside the cache sets the device error word (0xA01, 0xA02), its token is not
+ * appended, and with a bad position q is copied unturned.
+ */
+typedef struct MuseRopeAppend {
+  const void* q;            /* [tokens, heads, dim] */
+  const void* k;            /* [tokens, kv_heads, dim] */
+  const void* v;            /* [tokens, kv_heads, dim] */
+  void* q_out;              /* [tokens, heads, dim] */
+  void* k_pages;            /* [pages, kv_heads, page_size, dim], any page, head and entry strides */
+  void* v_pages;
+  const float* rope;        /* [positions, rotary]: rotary / 2 cosines, then rotary / 2 sines; contiguous */
+  const int32_t* position;  /* [tokens] */
+  const int64_t* slot;      /* [tokens] */
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, out_token, out_head;
+  int64_t k_page, k_page_head, k_entry, v_page, v_page_head, v_entry;
+  int64_t positions, pages;
+  int32_t tokens, heads, kv_heads, dim; /* dim 64 or 128 */
+  int32_t rotary;                       /* even, 2 .. dim */
+  int32_t page_size, interleaved, type; /* MUSE_BF16 or MUSE_F16 */
+} MuseRopeAppend;
+
+int muse_rope_append(const MuseRopeAppend* args, void* stream);
+
+/*
+ * Attention of each request's drafted tokens over its cached tokens and the drafted ones before them (a tree, a
+ * chain, or a single decoded token). Request b has tokens starts[b] .. starts[b + 1] - 1 (none is allowed), whose
+ * keys and values are already in the cache at entries context[b] + j. Every row sees the context; drafted token
+ * j where bit j % 32 of word j / 32 of its mask row is set (mask NULL: its own and every earlier one).
+ * out = softmax(scale * q . K) V over what the row sees, 0 where it sees nothing, times sigmoid(gate) if gate is
+ * given; FP32 softmax statistics and sums, rounded once. Entries of the cache that a row does not see, and what the
+ * pages hold past a request's tokens, never reach its result, whatever they hold.
+ * `scratch`: muse_tree_attention_scratch_bytes, not initialised, not shared by calls that overlap in time.
+ * Device error word: 0xB01 a request with more than max_draft tokens, 0xB02 a request past its page table,
+ * 0xB03 a page outside the cache; the requests concerned have unspecified results, the others are right.
+ */
+typedef struct MuseTreeAttention {
+  const void* q;            /* [tokens, heads, dim] */
+  const void* gate;         /* [tokens, heads, dim] or NULL */
+  void* out;                /* [tokens, heads, dim] */
+  const void* k_pages;      /* [pages, kv_heads, page_size, dim], any page, head and entry strides */
+  const void* v_pages;
+  const int32_t* table;     /* [requests, table_cols] page of each page_size entries */
+  const int32_t* context;   /* [requests] */
+  const int32_t* starts;    /* [requests + 1], starts[0] = 0, starts[requests] = tokens */
+  const uint32_t* mask;     /* [tokens, mask_words] or NULL */
+  void* scratch;
+  int64_t scratch_bytes;
+  int64_t q_token, q_head, gate_token, gate_head, out_token, out_head;
+  int64_t k_page, k_page_head, k_entry, v_page, v_page_head, v_entry;
+  int64_t table_row, mask_row, pages;
+  int32_t tokens, requests, max_draft; /* max_draft 1 .. 256: no request has more drafted tokens */
+  int32_t table_cols, mask_words;      /* 32 * mask_words >= max_draft */
+  int32_t heads, kv_heads, dim;        /* dim 64 or 128; heads a multiple of kv_heads */
+  int32_t page_size, type;             /* page_size a power of two, 8 .. 1024; MUSE_BF16 or MUSE_F16 */
+  float scale;
+} MuseTreeAttention;
+
+int muse_tree_attention(const MuseTreeAttention* args, void* stream);
+
+/* Scratch bytes of a muse_tree_attention call on the current device (reads only requests, max_draft, heads,
+ * kv_heads and dim of args). */
+int muse_tree_attention_scratch_bytes(const MuseTreeAttention* args, int64_t* bytes);
+
+/*
+ * The top_k experts of each token and their weights. Scores: softmax over the experts, or sigmoid. Choice: the
+ * logits without a bias, score + bias with one (the bias never enters a weight). groups > 1: experts
+ * g * experts / groups .. are group g, worth its best choice (with a bias: its best two added); only the best
+ * top_groups groups stay. Chosen in descending order, ties to the lowest index. weights = the chosen scores, divided
+ * by their sum if renormalize (0 where that is 0), times scale. A NaN logit counts as -inf; an expert of -inf is
+ * chosen after every other and weighs 0. `bias` is a constant: it may be read before the previous grid ends.
+ */
+typedef struct MuseRoute {
+  const void* logits;       /* [tokens, experts] */
+  const float* bias;        /* [experts] or NULL */
+  float* weights;           /* [tokens, top_k] contiguous */
+  int32_t* expert_ids;      /* [tokens, top_k] contiguous */
+  int64_t row;              /* row stride of logits */
+  int32_t tokens, experts;  /* experts 1 .. 1024 */
+  int32_t top_k;            /* 1 .. 32, at most the experts of top_groups groups */
+  int32_t groups, top_groups; /* groups divides experts, at most 32; 1 .. groups */
+  int32_t sigmoid, renormalize, type; /* MUSE_BF16, MUSE_F16 or MUSE_F32 */
+  float scale;
+} MuseRoute;
+
+int muse_route(const MuseRoute* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -77,6 +77,38 @@ class MuseGather(ctypes.Structure):
                 ("rank", ctypes.c_int32), ("ldy", ctypes.c_int64), ("col0", ctypes.c_int64)]
 
 
+
+TYPE_BF16, TYPE_F16, TYPE_F32 = 0, 1, 2
+
+
+class MuseRopeAppend(ctypes.Structure):
+    """Mirror of include/muse_proj.h MuseRopeAppend."""
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("q", "k", "v", "q_out", "k_pages", "v_pages", "rope", "position", "slot")] +
+                [(f, ctypes.c_int64) for f in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head", "out_token",
+                                               "out_head", "k_page", "k_page_head", "k_entry", "v_page", "v_page_head",
+                                               "v_entry", "positions", "pages")] +
+                [(f, ctypes.c_int32) for f in ("tokens", "heads", "kv_heads", "dim", "rotary", "page_size", "interleaved",
+                                               "type")])
+
+
+class MuseTreeAttention(ctypes.Structure):
+    """Mirror of include/muse_proj.h MuseTreeAttention."""
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("q", "gate", "out", "k_pages", "v_pages", "table", "context", "starts", "mask",
+                                                "scratch")] +
+                [(f, ctypes.c_int64) for f in ("scratch_bytes", "q_token", "q_head", "gate_token", "gate_head", "out_token",
+                                               "out_head", "k_page", "k_page_head", "k_entry", "v_page", "v_page_head",
+                                               "v_entry", "table_row", "mask_row", "pages")] +
+                [(f, ctypes.c_int32) for f in ("tokens", "requests", "max_draft", "table_cols", "mask_words", "heads",
+                                               "kv_heads", "dim", "page_size", "type")] + [("scale", ctypes.c_float)])
+
+
+class MuseRoute(ctypes.Structure):
+    """Mirror of include/muse_proj.h MuseRoute."""
+    _fields_ = ([(f, ctypes.c_void_p) for f in ("logits", "bias", "weights", "expert_ids")] + [("row", ctypes.c_int64)] +
+                [(f, ctypes.c_int32) for f in ("tokens", "experts", "top_k", "groups", "top_groups", "sigmoid", "renormalize",
+                                               "type")] + [("scale", ctypes.c_float)])
+
+
 _lib = None
 
 _P, _I64, _I32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
@@ -117,6 +149,10 @@ _SIGNATURES = {
     "muse_rows_bytes": ([_I64, _I64, _I32, ctypes.POINTER(_I64)], _I32),
     "muse_pack_rows": ([_P, _P, _I64, _I64, _I32, _P], _I32),
     "muse_proj_bf16_rows": ([_P, _P, _P, _I64, _I64, _I64, ctypes.POINTER(MusePlan), _P], _I32),
+    "muse_rope_append": ([ctypes.POINTER(MuseRopeAppend), _P], _I32),
+    "muse_tree_attention": ([ctypes.POINTER(MuseTreeAttention), _P], _I32),
+    "muse_tree_attention_scratch_bytes": ([ctypes.POINTER(MuseTreeAttention), ctypes.POINTER(_I64)], _I32),
+    "muse_route": ([ctypes.POINTER(MuseRoute), _P], _I32),
 }
 
 
@@ -344,3 +380,21 @@ def pack_rows(w_ptr: int, out_ptr: int, n: int, k: int, groups: int, stream: int
 
 def proj_bf16_rows(x_ptr: int, wrows_ptr: int, y_ptr: int, m: int, n: int, k: int, plan: MusePlan, stream: int) -> None:
     check(load().muse_proj_bf16_rows(x_ptr, wrows_ptr, y_ptr, m, n, k, ctypes.byref(plan), ctypes.c_void_p(stream)))
+
+
+def rope_append(args: MuseRopeAppend, stream: int) -> None:
+    check(load().muse_rope_append(args, stream))
+
+
+def tree_attention(args: MuseTreeAttention, stream: int) -> None:
+    check(load().muse_tree_attention(args, stream))
+
+
+def tree_attention_scratch_bytes(args: MuseTreeAttention) -> int:
+    out = ctypes.c_int64()
+    check(load().muse_tree_attention_scratch_bytes(args, ctypes.byref(out)))
+    return out.value
+
+
+def route(args: MuseRoute, stream: int) -> None:
+    check(load().muse_route(args, stream))

@@ -29,6 +29,9 @@
 #include "tc_pairk.cuh"
 #include "tc_pairsk.cuh"
 #include "gemv_tiles.cuh"
+#include "rope_append.cuh"
+#include "tree_attn.cuh"
+#include "route.cuh"
 
 #define MUSE_VERSION_STRING "muse_proj_b200 0.1 (sm_100a)"
 
@@ -1543,8 +1546,9 @@ int muse_device_error(int* code, void* stream) {
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e != cudaSuccess) return fail(MUSE_ERR_CUDA, "device_error: %s", cudaGetErrorString(e));
   *code = static_cast<int>(v);
-  if (v) return fail(MUSE_ERR_TIMEOUT, "device error word set (device code 0x%x: a bounded wait expired, or 0x501 an "
-                                        "escape of the device encoder outside its buffer)", v);
+  if (v) return fail(MUSE_ERR_TIMEOUT, "device error word set (device code 0x%x: a bounded wait expired, 0x501 an "
+                                        "escape of the device encoder outside its buffer, 0xa01, 0xa02 a position or "
+                                        "slot or 0xb01 .. 0xb03 a request or page out of its range)", v);
   return MUSE_OK;
 }
 
@@ -2238,3 +2242,7 @@ extern "C" int muse_proj_bf16_tiles_noalloc(const void* x, const void* tiles, vo
   return run_streamk(x, tiles, y, m, n, k, *plan, scratch, MUSE_NOALLOC_SCRATCH_BYTES,
                      static_cast<cudaStream_t>(stream));
 }
+
+// ---- operators between the projections ---------------------------------------------------------
+
+#include "serving.cuh"

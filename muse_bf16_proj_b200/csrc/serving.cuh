@@ -1,0 +1,208 @@
+// Host side of the operators between the projections: argument checks and launches (included by capi.cu).
+#pragma once
+
+namespace {
+
+// A kernel launch with programmatic dependent launch.
+template <typename K, typename... A>
+int launch_pdl(const char* what, K kern, dim3 grid, int threads, int smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, args...);
+  if (e != cudaSuccess) return fail(MUSE_ERR_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return MUSE_OK;
+}
+
+bool aligned_to(const void* p, unsigned n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+bool all_multiples(std::initializer_list<int64_t> v, int64_t n) {
+  for (int64_t x : v)
+    if (x % n) return false;
+  return true;
+}
+
+// Checks shared by the two cache operators: heads, dim, type and the cache's geometry.
+int check_heads(const char* op, int32_t heads, int32_t kv_heads, int32_t dim, int32_t type) {
+  if (heads < 1 || kv_heads < 1 || heads % kv_heads || heads > 4096)
+    return fail(MUSE_ERR_SHAPE, "%s: heads must be 1..4096 and a multiple of kv_heads (got %d and %d)", op, heads, kv_heads);
+  if (dim != 64 && dim != 128) return fail(MUSE_ERR_SHAPE, "%s: dim must be 64 or 128 (got %d)", op, dim);
+  if (type != MUSE_BF16 && type != MUSE_F16) return fail(MUSE_ERR_INVALID, "%s: type must be MUSE_BF16 or MUSE_F16 (got %d)", op, type);
+  return MUSE_OK;
+}
+
+}  // namespace
+
+extern "C" int muse_rope_append(const MuseRopeAppend* p, void* stream) {
+  muse::clear_error();
+  if (!p) return fail(MUSE_ERR_INVALID, "rope_append: null arguments");
+  if (p->tokens < 0) return fail(MUSE_ERR_INVALID, "rope_append: negative tokens");
+  if (int rc = check_heads("rope_append", p->heads, p->kv_heads, p->dim, p->type)) return rc;
+  if (p->rotary < 2 || p->rotary > p->dim || p->rotary % 2)
+    return fail(MUSE_ERR_SHAPE, "rope_append: rotary must be even, 2..dim (got %d)", p->rotary);
+  if (p->page_size < 1 || p->pages < 1 || p->positions < 1)
+    return fail(MUSE_ERR_INVALID, "rope_append: page_size, pages and positions must be positive");
+  if (p->tokens == 0) return MUSE_OK;
+  if (!p->q || !p->k || !p->v || !p->q_out || !p->k_pages || !p->v_pages || !p->rope || !p->position || !p->slot)
+    return fail(MUSE_ERR_INVALID, "rope_append: null pointer");
+  if (!aligned_to(p->q, 2) || !aligned_to(p->k, 2) || !aligned_to(p->v, 2) || !aligned_to(p->q_out, 2) ||
+      !aligned_to(p->k_pages, 2) || !aligned_to(p->v_pages, 2) || !aligned_to(p->rope, 4) || !aligned_to(p->position, 4) ||
+      !aligned_to(p->slot, 8))
+    return fail(MUSE_ERR_ALIGN, "rope_append: pointers must be aligned to their elements");
+  DeviceInfo* d;
+  if (int rc = device_info(&d)) return rc;
+  muse::RopeArgs a;
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.k = static_cast<const uint16_t*>(p->k);
+  a.v = static_cast<const uint16_t*>(p->v);
+  a.q_out = static_cast<uint16_t*>(p->q_out);
+  a.k_pages = static_cast<uint16_t*>(p->k_pages);
+  a.v_pages = static_cast<uint16_t*>(p->v_pages);
+  a.rope = p->rope;
+  a.position = p->position;
+  a.slot = p->slot;
+  a.q_token = p->q_token, a.q_head = p->q_head, a.k_token = p->k_token, a.k_head = p->k_head;
+  a.v_token = p->v_token, a.v_head = p->v_head, a.out_token = p->out_token, a.out_head = p->out_head;
+  a.kp_page = p->k_page, a.kp_head = p->k_page_head, a.kp_slot = p->k_entry;
+  a.vp_page = p->v_page, a.vp_head = p->v_page_head, a.vp_slot = p->v_entry;
+  a.positions = p->positions;
+  a.slots = p->pages * p->page_size;
+  a.tokens = p->tokens, a.heads = p->heads, a.kv_heads = p->kv_heads, a.dim = p->dim, a.rotary = p->rotary;
+  a.page = p->page_size, a.interleaved = p->interleaved ? 1 : 0;
+  const bool wide = p->rotary % 16 == 0 && aligned16(p->q) && aligned16(p->k) && aligned16(p->v) && aligned16(p->q_out) &&
+                    aligned16(p->k_pages) && aligned16(p->v_pages) && aligned16(p->rope) &&
+                    all_multiples({a.q_token, a.q_head, a.k_token, a.k_head, a.v_token, a.v_head, a.out_token, a.out_head,
+                                   a.kp_page, a.kp_head, a.kp_slot, a.vp_page, a.vp_head, a.vp_slot}, 8);
+  // Few tokens: more CTAs a token, down to one pass of its threads over the heads; many: one CTA a token.
+  const int64_t items = static_cast<int64_t>(a.heads + 2 * a.kv_heads) * (wide ? a.dim / 16 : a.dim / 2);
+  const int64_t passes = (items + muse::kRopeThreads - 1) / muse::kRopeThreads;
+  const int64_t split = std::min<int64_t>(passes, std::max<int64_t>(1, (8 * d->sms + a.tokens - 1) / a.tokens));
+  const dim3 grid(static_cast<unsigned>(a.tokens), static_cast<unsigned>(split), 1);
+  const bool half = p->type == MUSE_F16;
+  auto kern = wide ? (half ? muse::rope_append_kernel<true> : muse::rope_append_kernel<false>)
+                   : (half ? muse::rope_append_any_kernel<true> : muse::rope_append_any_kernel<false>);
+  return launch_pdl("rope_append", kern, grid, muse::kRopeThreads, 0, static_cast<cudaStream_t>(stream), a);
+}
+
+namespace {
+
+int check_attention(const MuseTreeAttention* p) {
+  if (!p) return fail(MUSE_ERR_INVALID, "tree_attention: null arguments");
+  if (int rc = check_heads("tree_attention", p->heads, p->kv_heads, p->dim, p->type)) return rc;
+  if (p->tokens < 0 || p->requests < 0) return fail(MUSE_ERR_INVALID, "tree_attention: negative tokens or requests");
+  if (p->max_draft < 1 || p->max_draft > 256)
+    return fail(MUSE_ERR_SHAPE, "tree_attention: max_draft must be 1..256 (got %d)", p->max_draft);
+  return MUSE_OK;
+}
+
+}  // namespace
+
+extern "C" int muse_tree_attention_scratch_bytes(const MuseTreeAttention* p, int64_t* bytes) {
+  muse::clear_error();
+  if (!bytes) return fail(MUSE_ERR_INVALID, "tree_attention_scratch_bytes: null output");
+  if (int rc = check_attention(p)) return rc;
+  *bytes = 16;
+  return MUSE_OK;
+}
+
+extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
+  muse::clear_error();
+  if (int rc = check_attention(p)) return rc;
+  if (p->page_size < 8 || p->page_size > 1024 || (p->page_size & (p->page_size - 1)))
+    return fail(MUSE_ERR_SHAPE, "tree_attention: page_size must be a power of two, 8..1024 (got %d)", p->page_size);
+  if (p->mask && static_cast<int64_t>(p->mask_words) * 32 < p->max_draft)
+    return fail(MUSE_ERR_SHAPE, "tree_attention: %d mask words do not cover max_draft %d", p->mask_words, p->max_draft);
+  if (p->pages < 1 || p->table_cols < 1) return fail(MUSE_ERR_INVALID, "tree_attention: pages and table_cols must be positive");
+  if (p->tokens == 0 || p->requests == 0) return MUSE_OK;
+  if (!p->q || !p->out || !p->k_pages || !p->v_pages || !p->table || !p->context || !p->starts || !p->scratch)
+    return fail(MUSE_ERR_INVALID, "tree_attention: null pointer");
+  if (!aligned16(p->q) || !aligned16(p->out) || !aligned16(p->k_pages) || !aligned16(p->v_pages) || !aligned16(p->gate) ||
+      !all_multiples({p->q_token, p->q_head, p->out_token, p->out_head, p->k_page, p->k_page_head, p->k_entry, p->v_page,
+                      p->v_page_head, p->v_entry}, 8) ||
+      (p->gate && !all_multiples({p->gate_token, p->gate_head}, 8)))
+    return fail(MUSE_ERR_ALIGN, "tree_attention: q, gate, out and the cache must be 16-byte aligned, rows included");
+  if (!aligned_to(p->table, 4) || !aligned_to(p->context, 4) || !aligned_to(p->starts, 4) || !aligned_to(p->mask, 4))
+    return fail(MUSE_ERR_ALIGN, "tree_attention: table, context, starts and mask must be 4-byte aligned");
+  DeviceInfo* d;
+  if (int rc = device_info(&d)) return rc;
+  muse::AttnArgs a;
+  a.q = static_cast<const uint16_t*>(p->q);
+  a.gate = static_cast<const uint16_t*>(p->gate);
+  a.k_pages = static_cast<const uint16_t*>(p->k_pages);
+  a.v_pages = static_cast<const uint16_t*>(p->v_pages);
+  a.out = static_cast<uint16_t*>(p->out);
+  a.table = p->table, a.context = p->context, a.starts = p->starts, a.mask = p->mask;
+  a.q_token = p->q_token, a.q_head = p->q_head, a.gate_token = p->gate_token, a.gate_head = p->gate_head;
+  a.out_token = p->out_token, a.out_head = p->out_head;
+  a.k_page = p->k_page, a.k_head = p->k_page_head, a.k_slot = p->k_entry;
+  a.v_page = p->v_page, a.v_head = p->v_page_head, a.v_slot = p->v_entry;
+  a.table_row = p->table_row, a.mask_row = p->mask_row, a.pages = p->pages;
+  a.requests = p->requests, a.tokens = p->tokens, a.max_draft = p->max_draft, a.table_cols = p->table_cols;
+  a.heads = p->heads, a.kv_heads = p->kv_heads, a.page = p->page_size;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  const bool half = p->type == MUSE_F16;
+  auto kern = p->dim == 64 ? (half ? muse::tree_attn_simple_kernel<true, 64> : muse::tree_attn_simple_kernel<false, 64>)
+                           : (half ? muse::tree_attn_simple_kernel<true, 128> : muse::tree_attn_simple_kernel<false, 128>);
+  const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
+  return launch_pdl("tree_attention", kern, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, static_cast<cudaStream_t>(stream), a);
+}
+
+namespace {
+
+template <int kType>
+int launch_route(const muse::RouteArgs& a, cudaStream_t st) {
+  const dim3 grid(static_cast<unsigned>((a.tokens + muse::kRouteWarps - 1) / muse::kRouteWarps));
+  const int threads = muse::kRouteWarps * 32;
+  if (a.count <= 128) return launch_pdl("route", muse::route_kernel<kType, 1>, grid, threads, 0, st, a);
+  if (a.count <= 256) return launch_pdl("route", muse::route_kernel<kType, 2>, grid, threads, 0, st, a);
+  if (a.count <= 512) return launch_pdl("route", muse::route_kernel<kType, 4>, grid, threads, 0, st, a);
+  return launch_pdl("route", muse::route_kernel<kType, 8>, grid, threads, 0, st, a);
+}
+
+}  // namespace
+
+extern "C" int muse_route(const MuseRoute* p, void* stream) {
+  muse::clear_error();
+  if (!p) return fail(MUSE_ERR_INVALID, "route: null arguments");
+  if (p->tokens < 0) return fail(MUSE_ERR_INVALID, "route: negative tokens");
+  if (p->experts < 1 || p->experts > muse::kRouteMaxExperts)
+    return fail(MUSE_ERR_SHAPE, "route: experts must be 1..%d (got %d)", muse::kRouteMaxExperts, p->experts);
+  if (p->groups < 1 || p->groups > muse::kRouteMaxGroups || p->experts % p->groups || p->top_groups < 1 || p->top_groups > p->groups)
+    return fail(MUSE_ERR_SHAPE, "route: groups must divide experts, 1..%d, and 1 <= top_groups <= groups (got %d, %d)",
+                muse::kRouteMaxGroups, p->groups, p->top_groups);
+  if (p->top_k < 1 || p->top_k > muse::kRouteMaxTopK || p->top_k > p->experts / p->groups * p->top_groups)
+    return fail(MUSE_ERR_SHAPE, "route: top_k must be 1..%d and at most the %d experts of top_groups groups (got %d)",
+                muse::kRouteMaxTopK, p->experts / p->groups * p->top_groups, p->top_k);
+  if (p->type != MUSE_BF16 && p->type != MUSE_F16 && p->type != MUSE_F32)
+    return fail(MUSE_ERR_INVALID, "route: type must be MUSE_BF16, MUSE_F16 or MUSE_F32 (got %d)", p->type);
+  if (p->tokens == 0) return MUSE_OK;
+  if (!p->logits || !p->weights || !p->expert_ids) return fail(MUSE_ERR_INVALID, "route: null pointer");
+  const int size = p->type == MUSE_F32 ? 4 : 2;
+  if (!aligned_to(p->logits, size) || !aligned_to(p->bias, 4) || !aligned_to(p->weights, 4) || !aligned_to(p->expert_ids, 4))
+    return fail(MUSE_ERR_ALIGN, "route: pointers must be aligned to their elements");
+  DeviceInfo* d;
+  if (int rc = device_info(&d)) return rc;
+  muse::RouteArgs a;
+  a.logits = p->logits;
+  a.bias = p->bias;
+  a.weights = p->weights;
+  a.experts = p->expert_ids;
+  a.row = p->row;
+  a.tokens = p->tokens, a.count = p->experts, a.top_k = p->top_k, a.groups = p->groups, a.top_groups = p->top_groups;
+  a.group_size = p->experts / p->groups;
+  a.group_magic = (1u << 20) / static_cast<unsigned>(a.group_size) + 1u;
+  a.sigmoid = p->sigmoid ? 1 : 0, a.renormalize = p->renormalize ? 1 : 0;
+  // Four logits a load where every lane's four are in one row and aligned together.
+  a.vector = p->experts % 4 == 0 && p->row % 4 == 0 && aligned_to(p->logits, static_cast<unsigned>(4 * size));
+  a.scale = p->scale;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p->type == MUSE_F32) return launch_route<muse::kRouteF32>(a, st);
+  if (p->type == MUSE_BF16) return launch_route<muse::kRouteBf16>(a, st);
+  return launch_route<muse::kRouteF16>(a, st);
+}
