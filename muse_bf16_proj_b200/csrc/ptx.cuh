@@ -42,8 +42,10 @@ __device__ __forceinline__ unsigned long long globaltimer() {
 
 __device__ __forceinline__ void report_error(unsigned int code) { atomicCAS(&g_dev_error, 0u, code); }
 
+// An argument out of its range (0xA01 .. 0xA0F, 0xB01 .. 0xB0F) concerns one token or request; nothing else stops for it.
 __device__ __forceinline__ bool error_raised() {
-  return *reinterpret_cast<volatile unsigned int*>(&g_dev_error) != 0u;
+  const unsigned int code = *reinterpret_cast<volatile unsigned int*>(&g_dev_error);
+  return code != 0u && !(code >= 0xA00u && (code & 0xF0u) == 0u);
 }
 
 // ---- per-CTA timestamp trace (off unless the host set a buffer) -----------------------------

@@ -101,13 +101,75 @@ int check_attention(const MuseTreeAttention* p) {
   return MUSE_OK;
 }
 
+int attention_rows(const MuseTreeAttention* p) {
+  // Rows that share a kv head, at most, rounded up to a row tile; past 128 several row tiles read the cache.
+  const int64_t rows = static_cast<int64_t>(p->max_draft) * (p->heads / p->kv_heads);
+  return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 128));
+}
+
+struct AttentionScratch {
+  int64_t ml, o, bytes;  // offsets of the partials' statistics and sums, and the whole
+};
+AttentionScratch attention_scratch(int64_t requests, int rows, int dim, int ctas) {
+  auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
+  AttentionScratch s;
+  s.ml = up((requests + 1) * 8);
+  s.o = s.ml + up(static_cast<int64_t>(ctas) * 2 * rows * 8);
+  s.bytes = s.o + static_cast<int64_t>(ctas) * 2 * rows * dim * 4;
+  return s;
+}
+
+// 4-D map of one cache tensor: dims, entries of a page, kv heads, pages; boxes of 64 dims x `box` entries.
+int make_cache_map(CUtensorMap* map, const void* base, const MuseTreeAttention* p, int64_t page, int64_t head, int64_t entry, int box) {
+  auto fn = encode_fn();
+  if (!fn) return fail(MUSE_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(p->dim), static_cast<cuuint64_t>(p->page_size), static_cast<cuuint64_t>(p->kv_heads),
+                        static_cast<cuuint64_t>(p->pages)};
+  cuuint64_t strides[3] = {static_cast<cuuint64_t>(entry * 2), static_cast<cuuint64_t>(head * 2), static_cast<cuuint64_t>(page * 2)};
+  cuuint32_t boxes[4] = {64u, static_cast<cuuint32_t>(box), 1u, 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  const CUresult r = fn(map, p->type == MUSE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                        const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(MUSE_ERR_CUDA, "cuTensorMapEncodeTiled of the cache failed (%d)", static_cast<int>(r));
+  return MUSE_OK;
+}
+
+template <bool kHalf, int kDim, int kRows>
+int launch_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas, cudaStream_t st) {
+  using Sh = muse::AttnShape<kDim, kRows>;
+  auto kern = muse::tree_attn_kernel<kHalf, kDim, kRows>;
+  static bool configured[kMaxDevices] = {};
+  int dev;
+  if (int rc = current_device(&dev)) return rc;
+  if (!configured[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    if (e != cudaSuccess) return fail(MUSE_ERR_CUDA, "cudaFuncSetAttribute(tree_attention): %s", cudaGetErrorString(e));
+    configured[dev] = true;
+  }
+  if (int rc = launch_pdl("tree_attention", kern, dim3(static_cast<unsigned>(ctas)), Sh::kThreads, Sh::kSmem, st, tmk, tmv, a)) return rc;
+  const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
+  return launch_pdl("tree_attention join", muse::tree_attn_join_kernel<kHalf, kDim, kRows>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128,
+                    0, st, a, ctas);
+}
+
+template <bool kHalf, int kDim>
+int launch_attention_rows(int rows, const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas, cudaStream_t st) {
+  if (rows == 16) return launch_attention<kHalf, kDim, 16>(tmk, tmv, a, ctas, st);
+  if (rows == 32) return launch_attention<kHalf, kDim, 32>(tmk, tmv, a, ctas, st);
+  if (rows == 64) return launch_attention<kHalf, kDim, 64>(tmk, tmv, a, ctas, st);
+  return launch_attention<kHalf, kDim, 128>(tmk, tmv, a, ctas, st);
+}
+
 }  // namespace
 
 extern "C" int muse_tree_attention_scratch_bytes(const MuseTreeAttention* p, int64_t* bytes) {
   muse::clear_error();
   if (!bytes) return fail(MUSE_ERR_INVALID, "tree_attention_scratch_bytes: null output");
   if (int rc = check_attention(p)) return rc;
-  *bytes = 16;
+  DeviceInfo* d;
+  if (int rc = device_info(&d)) return rc;
+  *bytes = attention_scratch(p->requests, attention_rows(p), p->dim, d->sms).bytes;
   return MUSE_OK;
 }
 
@@ -119,6 +181,8 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   if (p->mask && static_cast<int64_t>(p->mask_words) * 32 < p->max_draft)
     return fail(MUSE_ERR_SHAPE, "tree_attention: %d mask words do not cover max_draft %d", p->mask_words, p->max_draft);
   if (p->pages < 1 || p->table_cols < 1) return fail(MUSE_ERR_INVALID, "tree_attention: pages and table_cols must be positive");
+  if (static_cast<int64_t>(p->table_cols) * p->page_size > (int64_t(1) << 30) || p->pages > (int64_t(1) << 31) - 1)
+    return fail(MUSE_ERR_SHAPE, "tree_attention: a request's pages must hold at most 2^30 entries, the cache fewer than 2^31 pages");
   if (p->tokens == 0 || p->requests == 0) return MUSE_OK;
   if (!p->q || !p->out || !p->k_pages || !p->v_pages || !p->table || !p->context || !p->starts || !p->scratch)
     return fail(MUSE_ERR_INVALID, "tree_attention: null pointer");
@@ -129,8 +193,19 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
     return fail(MUSE_ERR_ALIGN, "tree_attention: q, gate, out and the cache must be 16-byte aligned, rows included");
   if (!aligned_to(p->table, 4) || !aligned_to(p->context, 4) || !aligned_to(p->starts, 4) || !aligned_to(p->mask, 4))
     return fail(MUSE_ERR_ALIGN, "tree_attention: table, context, starts and mask must be 4-byte aligned");
+  for (int64_t x : {p->k_page, p->k_page_head, p->k_entry, p->v_page, p->v_page_head, p->v_entry})
+    if (x < 0 || x >= (int64_t(1) << 38)) return fail(MUSE_ERR_SHAPE, "tree_attention: cache strides must be 0..2^38 (got %lld)", (long long)x);
   DeviceInfo* d;
   if (int rc = device_info(&d)) return rc;
+  const int tile = attention_rows(p);
+  const AttentionScratch sc = attention_scratch(p->requests, tile, p->dim, d->sms);
+  if (p->scratch_bytes < sc.bytes)
+    return fail(MUSE_ERR_CAPACITY, "tree_attention: needs %lld bytes of scratch (got %lld)", (long long)sc.bytes, (long long)p->scratch_bytes);
+  if (!aligned_to(p->scratch, 256)) return fail(MUSE_ERR_ALIGN, "tree_attention: scratch must be 256-byte aligned");
+  const int box = std::min(p->page_size, muse::kAttnTok);
+  CUtensorMap tmk, tmv;
+  if (int rc = make_cache_map(&tmk, p->k_pages, p, p->k_page, p->k_page_head, p->k_entry, box)) return rc;
+  if (int rc = make_cache_map(&tmv, p->v_pages, p, p->v_page, p->v_page_head, p->v_entry, box)) return rc;
   muse::AttnArgs a;
   a.q = static_cast<const uint16_t*>(p->q);
   a.gate = static_cast<const uint16_t*>(p->gate);
@@ -146,11 +221,17 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   a.requests = p->requests, a.tokens = p->tokens, a.max_draft = p->max_draft, a.table_cols = p->table_cols;
   a.heads = p->heads, a.kv_heads = p->kv_heads, a.page = p->page_size;
   a.scale_log2 = p->scale * 1.4426950408889634f;
-  const bool half = p->type == MUSE_F16;
-  auto kern = p->dim == 64 ? (half ? muse::tree_attn_simple_kernel<true, 64> : muse::tree_attn_simple_kernel<false, 64>)
-                           : (half ? muse::tree_attn_simple_kernel<true, 128> : muse::tree_attn_simple_kernel<false, 128>);
-  const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
-  return launch_pdl("tree_attention", kern, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, static_cast<cudaStream_t>(stream), a);
+  a.mask_words = p->mask_words;
+  uint8_t* base = static_cast<uint8_t*>(p->scratch);
+  a.prefix = reinterpret_cast<long long*>(base);
+  a.part_ml = reinterpret_cast<float2*>(base + sc.ml);
+  a.part_o = reinterpret_cast<float*>(base + sc.o);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (p->type == MUSE_F16)
+    return p->dim == 64 ? launch_attention_rows<true, 64>(tile, tmk, tmv, a, d->sms, st)
+                        : launch_attention_rows<true, 128>(tile, tmk, tmv, a, d->sms, st);
+  return p->dim == 64 ? launch_attention_rows<false, 64>(tile, tmk, tmv, a, d->sms, st)
+                      : launch_attention_rows<false, 128>(tile, tmk, tmv, a, d->sms, st);
 }
 
 namespace {
