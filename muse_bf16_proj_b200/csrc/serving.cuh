@@ -107,13 +107,17 @@ int attention_rows(const MuseTreeAttention* p) {
   return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 128));
 }
 
+int attention_tokens(int dim, int rows) {  // cached tokens a tile (AttnShape::kTok)
+  return dim == 64 && rows <= 32 ? 256 : 128;
+}
+
 struct AttentionScratch {
   int64_t ml, o, bytes;  // offsets of the partials' statistics and sums, and the whole
 };
-AttentionScratch attention_scratch(int64_t requests, int rows, int dim, int ctas) {
+AttentionScratch attention_scratch(int rows, int dim, int ctas) {
   auto up = [](int64_t x) { return (x + 255) / 256 * 256; };
   AttentionScratch s;
-  s.ml = up((requests + 1) * 8);
+  s.ml = up(static_cast<int64_t>(ctas) * sizeof(muse::AttnCross));
   s.o = s.ml + up(static_cast<int64_t>(ctas) * 2 * rows * 8);
   s.bytes = s.o + static_cast<int64_t>(ctas) * 2 * rows * dim * 4;
   return s;
@@ -148,9 +152,7 @@ int launch_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, const muse:
     configured[dev] = true;
   }
   if (int rc = launch_pdl("tree_attention", kern, dim3(static_cast<unsigned>(ctas)), Sh::kThreads, Sh::kSmem, st, tmk, tmv, a)) return rc;
-  const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
-  return launch_pdl("tree_attention join", muse::tree_attn_join_kernel<kHalf, kDim, kRows>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128,
-                    0, st, a, ctas);
+  return launch_pdl("tree_attention join", muse::tree_attn_join_kernel<kHalf, kDim, kRows>, dim3(static_cast<unsigned>(ctas), 16), 256, 0, st, a);
 }
 
 template <bool kHalf, int kDim>
@@ -169,7 +171,7 @@ extern "C" int muse_tree_attention_scratch_bytes(const MuseTreeAttention* p, int
   if (int rc = check_attention(p)) return rc;
   DeviceInfo* d;
   if (int rc = device_info(&d)) return rc;
-  *bytes = attention_scratch(p->requests, attention_rows(p), p->dim, d->sms).bytes;
+  *bytes = attention_scratch(attention_rows(p), p->dim, d->sms).bytes;
   return MUSE_OK;
 }
 
@@ -183,6 +185,10 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   if (p->pages < 1 || p->table_cols < 1) return fail(MUSE_ERR_INVALID, "tree_attention: pages and table_cols must be positive");
   if (static_cast<int64_t>(p->table_cols) * p->page_size > (int64_t(1) << 30) || p->pages > (int64_t(1) << 31) - 1)
     return fail(MUSE_ERR_SHAPE, "tree_attention: a request's pages must hold at most 2^30 entries, the cache fewer than 2^31 pages");
+  const int64_t tiles = static_cast<int64_t>(p->table_cols) * p->page_size / 128 + 1;
+  const int64_t units = static_cast<int64_t>(p->kv_heads) * (static_cast<int64_t>(p->max_draft) * (p->heads / p->kv_heads) / 128 + 1);
+  if (p->requests > 0 && tiles * units > ((int64_t(1) << 31) - 1) / p->requests)
+    return fail(MUSE_ERR_SHAPE, "tree_attention: requests x page table x kv_heads x max_draft is too large (more than 2^31 tiles)");
   if (p->tokens == 0 || p->requests == 0) return MUSE_OK;
   if (!p->q || !p->out || !p->k_pages || !p->v_pages || !p->table || !p->context || !p->starts || !p->scratch)
     return fail(MUSE_ERR_INVALID, "tree_attention: null pointer");
@@ -198,11 +204,11 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   DeviceInfo* d;
   if (int rc = device_info(&d)) return rc;
   const int tile = attention_rows(p);
-  const AttentionScratch sc = attention_scratch(p->requests, tile, p->dim, d->sms);
+  const AttentionScratch sc = attention_scratch(tile, p->dim, d->sms);
   if (p->scratch_bytes < sc.bytes)
     return fail(MUSE_ERR_CAPACITY, "tree_attention: needs %lld bytes of scratch (got %lld)", (long long)sc.bytes, (long long)p->scratch_bytes);
   if (!aligned_to(p->scratch, 256)) return fail(MUSE_ERR_ALIGN, "tree_attention: scratch must be 256-byte aligned");
-  const int box = std::min(p->page_size, muse::kAttnTok);
+  const int box = std::min(p->page_size, attention_tokens(p->dim, tile));
   CUtensorMap tmk, tmv;
   if (int rc = make_cache_map(&tmk, p->k_pages, p, p->k_page, p->k_page_head, p->k_entry, box)) return rc;
   if (int rc = make_cache_map(&tmv, p->v_pages, p, p->v_page, p->v_page_head, p->v_entry, box)) return rc;
@@ -222,8 +228,10 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   a.heads = p->heads, a.kv_heads = p->kv_heads, a.page = p->page_size;
   a.scale_log2 = p->scale * 1.4426950408889634f;
   a.mask_words = p->mask_words;
+  const unsigned int group = static_cast<unsigned int>(p->heads / p->kv_heads);
+  a.group_magic = group == 1 ? 0u : static_cast<unsigned int>(((uint64_t(1) << 32) + group - 1) / group);
   uint8_t* base = static_cast<uint8_t*>(p->scratch);
-  a.prefix = reinterpret_cast<long long*>(base);
+  a.cross = reinterpret_cast<muse::AttnCross*>(base);
   a.part_ml = reinterpret_cast<float2*>(base + sc.ml);
   a.part_o = reinterpret_cast<float*>(base + sc.o);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);

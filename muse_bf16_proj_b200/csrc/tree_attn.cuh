@@ -44,7 +44,6 @@ namespace muse {
 constexpr unsigned int kErrAttnDraft = 0xB01, kErrAttnTable = 0xB02, kErrAttnPage = 0xB03;
 constexpr unsigned int kErrAttnProducer = 0xB11, kErrAttnMma = 0xB12, kErrAttnSoftmax = 0xB13, kErrAttnDrain = 0xB14;
 
-constexpr int kAttnTok = 128;       // cached tokens a tile
 constexpr float kAttnSlack = 8.f;   // log2 of how far a score may pass its row's reference maximum
 constexpr float kAttnUnseen = -1e30f;  // reference of a row that has seen nothing: below every score, and finite
 
@@ -58,40 +57,57 @@ struct AttnArgs {
   long long table_row, mask_row;
   long long pages;
   int requests, tokens, max_draft, table_cols, heads, kv_heads, page, mask_words;
-  float scale_log2;  // scale * log2(e)
-  long long* prefix;  // scratch: [requests + 1] tiles before each request
-  float2* part_ml;    // scratch: [ctas][2][kRows] (reference maximum, sum)
-  float* part_o;      // scratch: [ctas][2][kRows][dim]
+  unsigned int group_magic;  // row / (heads / kv_heads) = umulhi(row, magic); 0: the group is one head
+  float scale_log2;          // scale * log2(e)
+  struct AttnCross* cross;   // scratch: [ctas]
+  float2* part_ml;           // scratch: [ctas][2][kRows] (reference maximum, sum)
+  float* part_o;             // scratch: [ctas][2][kRows][dim]
 };
 
-// Shared memory of a variant: K and V rings, Q, P, then the small arrays.
+// The row tile that starts in a CTA's run and goes on in the next ones: its rows, and the last run of it.
+struct AttnCross {
+  int first, row0, rows, head;  // request's first token, first row, rows (0: no such tile), kv head
+  int last, pad0, pad1, pad2;
+};
+static_assert(sizeof(AttnCross) == 32, "AttnCross layout");
+
+// (token of the request, head of the group) of a row.
+__device__ __forceinline__ int attn_token(const AttnArgs& a, int row) {
+  return a.group_magic ? static_cast<int>(__umulhi(static_cast<unsigned int>(row), a.group_magic)) : row;
+}
+
+// One variant: threads, rings, Q, P, then the small arrays in shared memory.
 template <int kDim, int kRows>
 struct AttnShape {
   static constexpr int kHalves = kDim / 64;
-  static constexpr int kStage = kAttnTok * kDim * 2;           // one K or V tile
+  static constexpr int kTG = kDim == 64 && kRows <= 32 ? 2 : 1;   // 128-token groups a tile
+  static constexpr int kCG = kRows <= 32 ? 1 : kRows / 32;        // column groups: at most 32 rows of Q a thread
+  static constexpr int kTok = 128 * kTG;                          // cached tokens a tile
+  static constexpr int kCols = kRows / kCG;
+  static constexpr int kSoft = 128 * kTG * kCG;                   // softmax threads
+  static constexpr int kThreads = 64 + kSoft;
+  static constexpr int kStage = kTok * kDim * 2;                  // one K or V tile
   static constexpr int kQ = kRows * kDim * 2;
-  static constexpr int kP = kAttnTok * kRows * 2;
+  static constexpr int kP = kTok * kRows * 2;
   static constexpr int kNP = kRows == 128 && kDim == 128 ? 1 : 2;  // P buffers
-  static constexpr int kNK = kDim == 64 ? (kRows <= 32 ? 6 : (kRows == 64 ? 5 : 4)) : (kRows <= 64 ? 3 : 2);
-  static constexpr int kNV = kDim == 64 ? kNK : (kRows <= 32 ? 3 : 2);
-  static constexpr int kGroups = kRows == 128 ? 2 : 1;         // softmax warpgroups, each its own columns
-  static constexpr int kCols = kRows / kGroups;                // columns (rows of Q) a group
-  static constexpr int kThreads = 64 + 128 * kGroups;
-  static constexpr int kTmem = kRows == 16 ? 64 : (kRows == 32 ? 128 : (kRows == 64 ? 256 : 512));
+  static constexpr int kNK = kDim == 64 ? (kRows <= 32 ? 3 : (kRows == 64 ? 5 : 4)) : (kRows <= 64 ? 3 : 2);
+  static constexpr int kNV = kDim == 64 ? (kRows == 32 ? 2 : kNK) : (kRows <= 32 ? 3 : 2);
+  static constexpr int kTmemO = 2 * kTG * kRows;                  // after two buffers of S^T
+  static constexpr int kTmem = kTmemO + kRows <= 64 ? 64 : (kTmemO + kRows <= 128 ? 128 : (kTmemO + kRows <= 256 ? 256 : 512));
   static constexpr int kOffV = kNK * kStage, kOffQ = kOffV + kNV * kStage, kOffP = kOffQ + kQ, kOffSmall = kOffP + kNP * kP;
-  // ref, rescale, 1 / sum and row ids [kRows]; red [4][kRows]; mask words [kRows][8]; barriers.
-  static constexpr int kSmall = kRows * 4 * 4 + 4 * kRows * 4 + kRows * 32 + (2 * kNK + 2 * kNV + 9) * 8 + 64;
+  // ref, rescale, 1 / sum and row ids [kRows]; red [4 kTG][kRows]; mask words [kRows][8]; barriers.
+  static constexpr int kSmall = kRows * 4 * 4 + 4 * kTG * kRows * 4 + kRows * 32 + (2 * kNK + 2 * kNV + 9) * 8 + 64;
   static constexpr int kSmem = 1024 + kOffSmall + kSmall;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 struct AttnReq {
   int first, drafted, ctx, kv, tiles, rows;  // first token, drafted tokens, context, entries, token tiles, rows a kv head
-  long long units;                           // kv heads x row tiles
+  int units;                                 // kv heads x row tiles
 };
 
 // A request's sizes, clamped to what may be touched whatever the device arrays hold.
-template <int kRows>
+template <int kTok, int kRows>
 __device__ __forceinline__ AttnReq attn_request(const AttnArgs& a, int b, bool report) {
   AttnReq r;
   const int lo = a.starts[b], hi = a.starts[b + 1], ctx = a.context[b];
@@ -104,47 +120,50 @@ __device__ __forceinline__ AttnReq attn_request(const AttnArgs& a, int b, bool r
   const long long have = static_cast<long long>(a.table_cols) * a.page, want = static_cast<long long>(r.ctx) + t;
   if (report && t > 0 && want > have) report_error(kErrAttnTable);
   r.kv = static_cast<int>(min(want, have));
-  r.tiles = t > 0 ? (r.kv + kAttnTok - 1) / kAttnTok : 0;
+  r.tiles = t > 0 ? (r.kv + kTok - 1) / kTok : 0;
   r.rows = t * (a.heads / a.kv_heads);
-  r.units = static_cast<long long>(a.kv_heads) * ((r.rows + kRows - 1) / kRows);
+  r.units = a.kv_heads * ((r.rows + kRows - 1) / kRows);
   return r;
 }
 
-// `total` tiles over at most `ctas` runs of at least one tile: how many runs, where run c starts, and
-// which run holds tile w (the largest c that starts at or before it).
-__device__ __forceinline__ int attn_runs(long long total, int ctas) { return static_cast<int>(min(total, static_cast<long long>(ctas))); }
-__device__ __forceinline__ long long attn_run_start(long long total, int c, int runs) { return total * c / runs; }
-__device__ __forceinline__ int attn_run_of(long long total, long long w, int runs) {
-  return static_cast<int>(((w + 1) * runs - 1) / total);
-}
+// `total` tiles over at most `ctas` runs of at least one tile, the first `more` one tile longer.
+struct AttnRuns {
+  int runs, per, more;
+  __device__ __forceinline__ AttnRuns(int total, int ctas) : runs(min(total, ctas)), per(0), more(0) {
+    if (runs > 0) per = total / runs, more = total - per * runs;
+  }
+  __device__ __forceinline__ int start(int c) const { return c * per + min(c, more); }
+  // The run that holds tile w.
+  __device__ __forceinline__ int of(int w) const {
+    const int longer = more * (per + 1);
+    return w < longer ? w / (per + 1) : more + (w - longer) / per;
+  }
+};
 
 // Walks a CTA's run segment by segment (a segment: consecutive token tiles of one row tile and kv head).
 struct AttnSeg {
   int b, head, row0, i0, i1;  // request, kv head, first row, token tiles [i0, i1)
-  long long unit0;            // tiles before this unit, over all requests
+  int unit0;                  // tiles before this unit, over all requests
   AttnReq r;
 };
-template <int kRows>
+template <int kTok, int kRows>
 struct AttnWalk {
-  long long left, base;  // tiles left in the run; tiles before request b
-  long long unit;
-  int b, i;
+  int left, base;  // tiles left in the run; tiles before request b
+  int unit, b, i;
   AttnReq r;
-  __device__ __forceinline__ AttnWalk(const AttnArgs& a, int b0, long long base0, long long w0, long long w1)
+  __device__ __forceinline__ AttnWalk(const AttnArgs& a, int b0, int base0, int w0, int w1)
       : left(w1 - w0), base(base0), unit(0), b(b0), i(0) {
-    if (left > 0) {
-      r = attn_request<kRows>(a, b, false);
-      const long long off = w0 - base;
-      unit = off / r.tiles;
-      i = static_cast<int>(off - unit * r.tiles);
-    }
+    r = attn_request<kTok, kRows>(a, b, false);
+    const int off = w0 - base;
+    unit = off / r.tiles;
+    i = off - unit * r.tiles;
   }
   __device__ __forceinline__ bool next(const AttnArgs& a, AttnSeg& s) {
     if (left <= 0) return false;
     while (unit >= r.units || r.tiles == 0) {
       base += r.units * r.tiles;
       if (++b >= a.requests) return false;
-      r = attn_request<kRows>(a, b, false);
+      r = attn_request<kTok, kRows>(a, b, false);
       unit = 0;
       i = 0;
     }
@@ -152,11 +171,11 @@ struct AttnWalk {
     s.r = r;
     // Row tiles of one kv head follow one another, so that CTAs that share cached tokens run side by side.
     const int row_tiles = (r.rows + kRows - 1) / kRows;
-    s.head = static_cast<int>(unit / row_tiles);
-    s.row0 = static_cast<int>(unit % row_tiles) * kRows;
+    s.head = row_tiles == 1 ? unit : unit / row_tiles;
+    s.row0 = (unit - s.head * row_tiles) * kRows;
     s.unit0 = base + unit * r.tiles;
     s.i0 = i;
-    s.i1 = static_cast<int>(min(static_cast<long long>(r.tiles), i + left));
+    s.i1 = min(r.tiles, i + left);
     left -= s.i1 - s.i0;
     ++unit;
     i = 0;
@@ -228,29 +247,24 @@ __device__ __forceinline__ void add16x2(uint32_t p, float& lo, float& hi) {
   }
 }
 
-// kN (32 or 16) values a lane reduced over the warp's lanes by halving: afterwards lane l holds column l
-// (32) or l / 2 (16) in v[0].
-template <int kN, bool kMax>
-__device__ __forceinline__ void warp_fold(float* v, int lane) {
-  int n = kN;
+// 16 values a lane reduced over the warp's lanes by halving (16 shuffles in all): afterwards lane l holds
+// column l / 2 in v[0].
+template <bool kMax>
+__device__ __forceinline__ void warp_fold16(float* v, int lane) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    if (n > 1) {
-      n >>= 1;
-      const bool up = (lane & o) != 0;
+  for (int n = 8, o = 16; n; n >>= 1, o >>= 1) {
+    const bool up = (lane & o) != 0;
 #pragma unroll
-      for (int j = 0; j < kN / 2; ++j) {
-        if (j < n) {
-          const float give = up ? v[j] : v[j + n], keep = up ? v[j + n] : v[j];
-          const float got = __shfl_xor_sync(0xffffffffu, give, o);
-          v[j] = kMax ? fmaxf(keep, got) : keep + got;
-        }
+    for (int j = 0; j < 8; ++j) {
+      if (j < n) {
+        const float give = up ? v[j] : v[j + n], keep = up ? v[j + n] : v[j];
+        const float got = __shfl_xor_sync(0xffffffffu, give, o);
+        v[j] = kMax ? fmaxf(keep, got) : keep + got;
       }
-    } else {
-      const float got = __shfl_xor_sync(0xffffffffu, v[0], o);
-      v[0] = kMax ? fmaxf(v[0], got) : v[0] + got;
     }
   }
+  const float got = __shfl_xor_sync(0xffffffffu, v[0], 1);
+  v[0] = kMax ? fmaxf(v[0], got) : v[0] + got;
 }
 
 // UMMA descriptor of an M- or N-major 16-bit operand: `row` bytes of M/N entries a k row (swizzled at that width),
@@ -264,7 +278,9 @@ template <bool kHalf, int kDim, int kRows>
 __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttnArgs a) {
   using Sh = AttnShape<kDim, kRows>;
-  constexpr int kHalves = Sh::kHalves, kNK = Sh::kNK, kNV = Sh::kNV, kNP = Sh::kNP, kCols = Sh::kCols;
+  using Walk = AttnWalk<Sh::kTok, kRows>;
+  constexpr int kHalves = Sh::kHalves, kNK = Sh::kNK, kNV = Sh::kNV, kNP = Sh::kNP, kCols = Sh::kCols, kTok = Sh::kTok;
+  constexpr int kTG = Sh::kTG, kSoft = Sh::kSoft;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_align<1024>(smem_raw);
   uint8_t* ring_k = smem;
@@ -275,8 +291,8 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   float* rescale = ref + kRows;
   float* inv = rescale + kRows;
   int* row_id = reinterpret_cast<int*>(inv + kRows);             // token of the request << 16 | query head
-  float* red = reinterpret_cast<float*>(row_id + kRows);         // [4][kRows]
-  uint32_t* words = reinterpret_cast<uint32_t*>(red + 4 * kRows);  // [kRows][8]: drafted tokens a row sees
+  float* red = reinterpret_cast<float*>(row_id + kRows);         // [4 kTG][kRows]
+  uint32_t* words = reinterpret_cast<uint32_t*>(red + 4 * kTG * kRows);  // [kRows][8]: drafted tokens a row sees
   uint64_t* k_full = reinterpret_cast<uint64_t*>(words + kRows * 8);
   uint64_t* k_empty = k_full + kNK;
   uint64_t* v_full = k_empty + kNK;
@@ -288,9 +304,9 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   uint64_t* pv_done = p_full + 2;
   uint64_t* q_full = pv_done + 2;
   uint64_t* fin = q_full + 1;
-  long long* start_s = reinterpret_cast<long long*>(fin + 1);  // first request's tiles before it
-  int* start_b = reinterpret_cast<int*>(start_s + 1);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start_b + 1);
+  int* start_b = reinterpret_cast<int*>(fin + 1);  // the run's first request, and the tiles before it
+  int* start_s = start_b + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start_s + 1);
   int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);  // a drafted token of this segment has a non-finite V entry
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -299,73 +315,73 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     prefetch_tensormap(&tmv);
     for (int i = 0; i < kNK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
     for (int i = 0; i < kNV; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 128 * Sh::kGroups), mbar_init(&pv_done[i], 1);
-    mbar_init(q_full, 128 * Sh::kGroups);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kSoft), mbar_init(&pv_done[i], 1);
+    mbar_init(q_full, kSoft);
     mbar_init(fin, 1);
     fence_mbar_init();
-    *start_b = a.requests;
-    *odd_v = 0;
   }
   if (warp == 1) tmem_alloc(tmem_slot, Sh::kTmem);
   pdl_launch_dependents();
   pdl_wait();
 
   // Tiles before each request: a scan over the requests by the whole CTA, a run of requests a thread.
-  long long total = 0, before = 0;
+  int total = 0, before = 0, mine = 0;
   const int each = (a.requests + Sh::kThreads - 1) / Sh::kThreads;
   const int b_lo = min(static_cast<int>(threadIdx.x) * each, a.requests), b_hi = min(b_lo + each, a.requests);
   {
-    long long* sums = reinterpret_cast<long long*>(red);
-    long long mine = 0;
+    int* sums = reinterpret_cast<int*>(red);
+    int only = 0;
     for (int b = b_lo; b < b_hi; ++b) {
-      const AttnReq r = attn_request<kRows>(a, b, blockIdx.x == 0);
-      mine += r.units * r.tiles;
+      const AttnReq r = attn_request<kTok, kRows>(a, b, blockIdx.x == 0);
+      only = r.units * r.tiles;
+      mine += only;
     }
-    long long upto = mine;
+    int upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += x;
     }
     if (lane == 31) sums[warp] = upto;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < Sh::kThreads / 32; ++w) {
       if (w < warp) before += sums[w];
       total += sums[w];
     }
     before += upto - mine;
-    __syncthreads();
   }
-  const int runs = attn_runs(total, gridDim.x);
-  long long w0 = 0, w1 = 0;
-  if (static_cast<int>(blockIdx.x) < runs) w0 = attn_run_start(total, blockIdx.x, runs), w1 = attn_run_start(total, blockIdx.x + 1, runs);
-  {
-    long long at = before;
-    for (int b = b_lo; b < b_hi; ++b) {
-      const AttnReq r = attn_request<kRows>(a, b, false);
-      if (blockIdx.x == 0) a.prefix[b] = at;
-      const long long end = at + r.units * r.tiles;
-      if (at <= w0 && w0 < end) *start_s = at, *start_b = b;
-      at = end;
+  const AttnRuns runs(total, gridDim.x);
+  const bool work = static_cast<int>(blockIdx.x) < runs.runs;
+  const int w0 = work ? runs.start(blockIdx.x) : 0, w1 = work ? runs.start(blockIdx.x + 1) : 0;
+  if (work && before <= w0 && w0 < before + mine) {
+    int at = before, b = b_lo;
+    if (each > 1) {
+      for (;; ++b) {
+        const AttnReq r = attn_request<kTok, kRows>(a, b, false);
+        if (w0 < at + r.units * r.tiles) break;
+        at += r.units * r.tiles;
+      }
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.prefix[a.requests] = total;
+    *start_s = at, *start_b = b;
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int b0 = *start_b;
-  const bool work = w0 < w1 && b0 < a.requests;
-  const uint32_t tmem_o = tmem + 2 * kRows;
+  const int b0 = *start_b, s0 = *start_s;
+  const uint32_t tmem_o = tmem + Sh::kTmemO;
 
   if (warp == 0) {
     // ---- producer: lane = one box ------------------------------------------------------------------
     if (work) {
+      static_assert(kTok / 8 * kHalves <= 32, "a lane a box");
       int issued_k = 0, issued_v = 0;
-      AttnWalk<kRows> walk(a, b0, *start_s, w0, w1);
+      Walk walk(a, b0, s0, w0, w1);
       AttnSeg s;
-      const int box = min(a.page, kAttnTok), boxes = kAttnTok / box;
-      const int mine = lane % boxes, half = lane / boxes;  // this lane's box of the tile and 64-dim half
+      const int box = min(a.page, kTok), boxes = kTok / box;
+      const int half = lane / boxes, num = lane - half * boxes;  // 64-dim half and place of this lane's box
+      const uint32_t off = static_cast<uint32_t>(half * (kTok * 128) + num * box * 128);
       // Tokens that several row tiles read stay in L2; a request's only reader streams them.
       const uint64_t stream = policy_evict_first(), keep = policy_evict_normal();
       Ring rk, rv;
@@ -376,18 +392,17 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         int page = 0;
         bool have = false;
         auto lookup = [&](int i) {
-          const int pos = i * kAttnTok + mine * box;
+          const int pos = i * kTok + num * box;
           have = half < kHalves && pos < s.r.kv;
-          page = have ? row[pos / a.page] : 0;
+          page = have ? row[static_cast<unsigned int>(pos) / static_cast<unsigned int>(a.page)] : 0;
         };
         lookup(s.i0);
         for (int i = s.i0; i < s.i1; ++i) {
-          const int now = page, in = (i * kAttnTok + mine * box) % a.page;
+          const int now = page, in = (i * kTok + num * box) & (a.page - 1);
           const bool go = have;
           if (go && (now < 0 || now >= a.pages)) report_error(kErrAttnPage);  // reads as zeros: outside the map
           if (i + 1 < s.i1) lookup(i + 1);
           const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, go)) * box * 128);
-          const uint32_t off = static_cast<uint32_t>(half * (kAttnTok * 128) + mine * box * 128);
           ok = mbar_wait(&k_empty[rk.slot], rk.phase ^ 1u, kErrAttnProducer);
           if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
           if (lane == 0) mbar_expect_tx(&k_full[rk.slot], bytes);
@@ -413,14 +428,14 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   } else if (warp == 1) {
     // ---- UMMA issue --------------------------------------------------------------------------------
     if (work && lane == 0) {
-      AttnWalk<kRows> walk(a, b0, *start_s, w0, w1);
+      Walk walk(a, b0, s0, w0, w1);
       AttnSeg s;
       constexpr uint32_t kType = kHalf ? 0u : ((1u << 7) | (1u << 10));
       constexpr uint32_t kShape = (1u << 4) | (static_cast<uint32_t>(kRows >> 3) << 17) | (8u << 24);
       constexpr uint32_t idesc_s = kShape | kType, idesc_o = kShape | kType | (1u << 15) | (1u << 16);
       constexpr int kPRow = kRows >= 64 ? 128 : kRows * 2;  // bytes of a token's row of P
-      constexpr uint64_t v_bits = attn_mn_desc_bits(128, kDim == 128 ? kAttnTok * 128 : 0);
-      constexpr uint64_t p_bits = attn_mn_desc_bits(kPRow, kRows == 128 ? kAttnTok * 128 : 0);
+      constexpr uint64_t v_bits = attn_mn_desc_bits(128, kDim == 128 ? kTok * 128 : 0);
+      constexpr uint64_t p_bits = attn_mn_desc_bits(kPRow, kRows == 128 ? kTok * 128 : 0);
       Ring rk, rv;
       uint32_t seg_phase = 0, n = 0;
       bool ok = true;
@@ -429,11 +444,13 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         tc_fence_after();
         const uint64_t dk = umma_desc_sw128(smem_u32(ring_k + rk.slot * Sh::kStage)), dq = umma_desc_sw128(smem_u32(q_s));
 #pragma unroll
-        for (int h = 0; h < kHalves; ++h)
+        for (int t = 0; t < kTG; ++t)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16(tmem + (m & 1u) * kRows, dk + ((h * kAttnTok * 128) >> 4) + 2 * k, dq + ((h * kRows * 128) >> 4) + 2 * k, idesc_s,
-                      (h | k) != 0);
+          for (int h = 0; h < kHalves; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_bf16(tmem + ((m & 1u) * kTG + t) * kRows, dk + ((h * kTok * 128 + t * 128 * 128) >> 4) + 2 * k,
+                        dq + ((h * kRows * 128) >> 4) + 2 * k, idesc_s, (h | k) != 0);
         umma_commit(&k_empty[rk.slot]);
         umma_commit(&s_full[m & 1u]);
         rk.next(kNK);
@@ -454,7 +471,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           const uint64_t dv = v_bits | ((smem_u32(ring_v + rv.slot * Sh::kStage) & 0x3FFFFu) >> 4);
           const uint64_t dp = p_bits | ((smem_u32(p_s + (n % kNP) * Sh::kP) & 0x3FFFFu) >> 4);
 #pragma unroll
-          for (int k = 0; k < kAttnTok / 16; ++k)
+          for (int k = 0; k < kTok / 16; ++k)
             umma_bf16(tmem_o, dv + ((k * 16 * 128) >> 4), dp + ((k * 16 * kPRow) >> 4), idesc_o, (i > s.i0 || k > 0) ? 1u : 0u);
           umma_commit(&v_empty[rv.slot]);
           umma_commit(&pv_done[n & 1u]);
@@ -465,269 +482,302 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       mbar_wait(fin, 0u, kErrAttnDrain, kWaitLimitNs / 10);  // nothing of the tensor cores is under way past here
     }
     __syncwarp();
-  } else if (work) {
-    // ---- softmax: thread = one token of the tile (TMEM lane), all columns of its group --------------
-    const int tid = static_cast<int>(threadIdx.x) - 64, group = tid >> 7;
-    const int quarter = warp & 3, token = quarter * 32 + lane, gtid = tid & 127;
-    const int c0 = group * kCols;
-    const int bar = 1 + group;
-    constexpr int kAll = 128 * Sh::kGroups;
+  } else {
+    // ---- softmax: thread = one token of the tile (a TMEM lane of its token group), its group's columns ----
+    const int tid = static_cast<int>(threadIdx.x) - 64;
+    const int tg = (tid >> 7) % kTG, cg = (tid >> 7) / kTG;
+    const int quarter = warp & 3, tl = quarter * 32 + lane, token = tg * 128 + tl;
+    const int c0 = cg * kCols;
+    const int bar = 1 + cg;
+    constexpr int kGroup = 128 * kTG;  // threads that share columns
+    const int gtid = tid % kGroup;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const int g = a.heads / a.kv_heads;
     const float kNegInf = __int_as_float(0xff800000);
     const float c = a.scale_log2;
-    AttnWalk<kRows> walk(a, b0, *start_s, w0, w1);
-    AttnSeg s;
-    uint32_t n = 0;  // tiles done in this run
-    uint32_t v_slot = 0, v_phase = 0;
-    bool ok = true;
-    float l[kCols];
-    while (ok && walk.next(a, s)) {
-      // ---- the segment's rows: Q, mask words, references -------------------------------------------
-      const int rows = min(kRows, s.r.rows - s.row0);
-      const int full = min(kRows, (rows + 15) & ~15);  // columns that are computed
-      const int live = min(max(full - c0, 0), kCols);  // of this group
-      bar_named(3, kAll);                              // every thread is done with the last segment's arrays
-      for (int i = tid; i < full * (kDim / 8); i += kAll) {
-        const int r = i / (kDim / 8), ch = i % (kDim / 8);
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows) {
-          const int row = s.row0 + r, t = row / g;
-          v = ldg_cg_v4(a.q + (s.r.first + t) * a.q_token + (s.head * g + row - t * g) * a.q_head + ch * 8);
-        }
-        const uint32_t at = smem_u32(q_s) + (ch >> 3) * (kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
-        st_shared_v4u(at, v.x, v.y, v.z, v.w);
-      }
-      const int nw = (s.r.drafted + 31) >> 5;
-      for (int i = tid; i < full * nw; i += kAll) {
-        const int r = i / nw, w = i - r * nw;
-        uint32_t v = 0u;
-        if (r < rows) {
-          const int t = (s.row0 + r) / g;
-          // Bits up to the token itself without a mask; nothing past the request's tokens.
-          const int last = a.mask ? s.r.drafted : t + 1;
-          v = a.mask ? a.mask[(s.r.first + t) * a.mask_row + w] : 0xffffffffu;
-          const int nb = min(last, s.r.drafted) - w * 32;
-          v &= nb >= 32 ? 0xffffffffu : (nb <= 0 ? 0u : (1u << nb) - 1u);
-        }
-        words[r * 8 + w] = v;
-      }
-      if (tid < kRows) {
-        const int row = min(s.row0 + tid, s.r.rows - 1), t = row / g;
-        ref[tid] = kAttnUnseen;
-        row_id[tid] = (t << 16) | (s.head * g + row - t * g);
-      }
-      if (tid == 0) *odd_v = 0;
-      fence_proxy_async_shared();
-      mbar_arrive(q_full);
-      bar_named(3, kAll);
+    AttnCross cross = {};
+    if (work) {
+      Walk walk(a, b0, s0, w0, w1);
+      AttnSeg s;
+      uint32_t n = 0;  // tiles done in this run
+      uint32_t v_slot = 0, v_phase = 0;
+      bool ok = true;
+      float l[kCols];
+      while (ok && walk.next(a, s)) {
+        // ---- the segment's rows: Q, mask words, references -----------------------------------------
+        const int rows = min(kRows, s.r.rows - s.row0);
+        const int full = min(kRows, (rows + 15) & ~15);  // columns that are computed
+        const int live = min(max(full - c0, 0), kCols);  // of this group
+        bar_named(8, kSoft);                             // every thread is done with the last segment's arrays
+        constexpr int kLoads = kRows * (kDim / 8) / kSoft > 0 ? kRows * (kDim / 8) / kSoft : 1;
+        uint4 qv[kLoads];
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) l[j] = 0.f;
+        for (int u = 0; u < kLoads; ++u) {
+          const int i = tid + u * kSoft, r = i / (kDim / 8), ch = i % (kDim / 8);
+          qv[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < rows) {
+            const int t = attn_token(a, s.row0 + r);
+            qv[u] = __ldg(reinterpret_cast<const uint4*>(a.q + (s.r.first + t) * a.q_token +
+                                                         (s.head * g + s.row0 + r - t * g) * a.q_head + ch * 8));
+          }
+        }
+        // Drafted tokens that each row sees: bits up to itself without a mask; nothing past the request's tokens.
+        const int nw = (s.r.drafted + 31) >> 5;
+        for (int i = tid; i < full * 8; i += kSoft) {
+          const int r = i >> 3, w = i & 7;
+          if (w < nw) {
+            uint32_t v = 0u;
+            if (r < rows) {
+              const int t = attn_token(a, s.row0 + r);
+              v = a.mask ? a.mask[(s.r.first + t) * a.mask_row + w] : 0xffffffffu;
+              const int nb = (a.mask ? s.r.drafted : min(t + 1, s.r.drafted)) - w * 32;
+              v &= nb >= 32 ? 0xffffffffu : (nb <= 0 ? 0u : (1u << nb) - 1u);
+            }
+            words[i] = v;
+          }
+        }
+        if (tid < kRows) {
+          const int row = min(s.row0 + tid, s.r.rows - 1), t = attn_token(a, row);
+          ref[tid] = kAttnUnseen;
+          row_id[tid] = (t << 16) | (s.head * g + row - t * g);
+        }
+        if (tid == 0) *odd_v = 0;
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+          const int i = tid + u * kSoft, r = i / (kDim / 8), ch = i % (kDim / 8);
+          if (r < full)
+            st_shared_v4u(smem_u32(q_s) + (ch >> 3) * (kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), qv[u].x, qv[u].y, qv[u].z,
+                          qv[u].w);
+        }
+        fence_proxy_async_shared();
+        mbar_arrive(q_full);
+        bar_named(8, kSoft);
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) l[j] = 0.f;
+        const bool lone = s.r.drafted == 1 && !a.mask;  // one token, which sees itself
 
-      // ---- tiles -----------------------------------------------------------------------------------
-      for (int i = s.i0; ok && i < s.i1; ++i, ++n) {
-        ok = mbar_wait(&s_full[n & 1u], (n >> 1) & 1u, kErrAttnSoftmax);
-        // P's buffer is free, and with two of them PV of two tiles ago is done, once this has passed.
-        if (n >= static_cast<uint32_t>(kNP)) ok = mbar_wait(&pv_done[(n - kNP) & 1u], ((n - kNP) >> 1) & 1u, kErrAttnSoftmax) && ok;
-        tc_fence_after();
-        float x[kCols];
-        const uint32_t ts = tmem + (n & 1u) * kRows + c0 + lanes;
+        // ---- tiles ---------------------------------------------------------------------------------
+        for (int i = s.i0; ok && i < s.i1; ++i, ++n) {
+          ok = mbar_wait(&s_full[n & 1u], (n >> 1) & 1u, kErrAttnSoftmax);
+          // P's buffer is free, and with two of them PV of two tiles ago is done, once this has passed.
+          if (n >= static_cast<uint32_t>(kNP)) ok = mbar_wait(&pv_done[(n - kNP) & 1u], ((n - kNP) >> 1) & 1u, kErrAttnSoftmax) && ok;
+          tc_fence_after();
+          float x[kCols];
+          const uint32_t ts = tmem + ((n & 1u) * kTG + tg) * kRows + c0 + lanes;
 #pragma unroll
-        for (int cc = 0; cc < kCols; cc += 16)
-          if (cc < live) attn_ld16(ts + cc, x + cc);
+          for (int cc = 0; cc < kCols; cc += 16)
+            if (cc < live) attn_ld16(ts + cc, x + cc);
 #pragma unroll
-        for (int cc = 0; cc < kCols; cc += 16)
-          if (cc < live) attn_ld_wait(x + cc);
-        const int pos = i * kAttnTok + token;
-        const bool edge = (i + 1) * kAttnTok > s.r.ctx;  // the tile reaches past the context
-        const float cm = edge ? 1.f : c;                 // scores of an edge tile are scaled here, with their mask
-        if (edge) {
-          const int j = pos - s.r.ctx;
+          for (int cc = 0; cc < kCols; cc += 16)
+            if (cc < live) attn_ld_wait(x + cc);
+          const int pos = i * kTok + token;
+          const bool edge = (i + 1) * kTok > s.r.ctx;  // the tile reaches past the context
+          const float cm = edge ? 1.f : c;             // scores of an edge tile are scaled here, with their mask
+          if (edge) {
+            // Bit k: this token is seen by column k.
+            uint32_t seen = pos < s.r.kv ? 0xffffffffu : 0u;
+            const int j = pos - s.r.ctx;
+            if (!lone && seen && j >= 0) {
+              seen = 0u;
 #pragma unroll
-          for (int k = 0; k < kCols; ++k) {
-            if (k < live) {
-              const bool seen = j < 0 || (pos < s.r.kv && ((words[(c0 + k) * 8 + (j >> 5)] >> (j & 31)) & 1u));
-              x[k] = seen ? x[k] * c : kNegInf;
+              for (int k = 0; k < kCols; ++k)
+                if (k < live) seen |= ((words[(c0 + k) * 8 + (j >> 5)] >> (j & 31)) & 1u) << k;
+            }
+#pragma unroll
+            for (int k = 0; k < kCols; ++k) x[k] = (seen >> k) & 1u ? x[k] * c : kNegInf;
+          }
+          bool past = false;
+#pragma unroll
+          for (int cc = 0; cc < kCols; cc += 4) {
+            if (cc < live) {
+              const float4 m = *reinterpret_cast<const float4*>(ref + c0 + cc);
+              past |= fmaf(x[cc], cm, -m.x) > kAttnSlack;
+              past |= fmaf(x[cc + 1], cm, -m.y) > kAttnSlack;
+              past |= fmaf(x[cc + 2], cm, -m.z) > kAttnSlack;
+              past |= fmaf(x[cc + 3], cm, -m.w) > kAttnSlack;
             }
           }
-        }
-        bool past = false;
-#pragma unroll
-        for (int cc = 0; cc < kCols; cc += 4) {
-          if (cc < live) {
-            const float4 m = *reinterpret_cast<const float4*>(ref + c0 + cc);
-            past |= fmaf(x[cc], cm, -m.x) > kAttnSlack;
-            past |= fmaf(x[cc + 1], cm, -m.y) > kAttnSlack;
-            past |= fmaf(x[cc + 2], cm, -m.z) > kAttnSlack;
-            past |= fmaf(x[cc + 3], cm, -m.w) > kAttnSlack;
-          }
-        }
-        if (bar_any(bar, 128, past || !ok)) {
-          if (bar_any(bar, 128, !ok)) {
-            ok = false;
-            break;
-          }
-          // Move the references to the true maxima and rescale what was summed against the old ones.
-          constexpr int kFold = kCols < 32 ? kCols : 32;
-#pragma unroll
-          for (int cc = 0; cc < kCols; cc += kFold) {
-            float top[kFold];
-#pragma unroll
-            for (int j = 0; j < kFold; ++j) top[j] = cc + j < live ? x[cc + j] * cm : kNegInf;
-            warp_fold<kFold, true>(top, lane);
-            if (kFold == 32 || !(lane & 1)) red[quarter * kRows + c0 + cc + (kFold == 32 ? lane : lane >> 1)] = top[0];
-          }
-          bar_named(bar, 128);
-          if (gtid < kCols) {
-            const int col = c0 + gtid;
-            const float old = ref[col];
-            const float now = fmaxf(fmaxf(fmaxf(red[col], red[kRows + col]), fmaxf(red[2 * kRows + col], red[3 * kRows + col])), old);
-            ref[col] = now;
-            rescale[col] = ex2(old - now);
-          }
-          bar_named(bar, 128);
-#pragma unroll
-          for (int j = 0; j < kCols; ++j)
-            if (j < live) l[j] *= rescale[c0 + j];
-          if (i > s.i0) {
-            ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax);
-            tc_fence_after();
+          if (bar_any(bar, kGroup, past || !ok)) {
+            if (bar_any(bar, kGroup, !ok)) {
+              ok = false;
+              break;
+            }
+            // Move the references to the true maxima and rescale what was summed against the old ones.
 #pragma unroll
             for (int cc = 0; cc < kCols; cc += 16) {
-              if (cc < live) {
-                float o[16];
-                attn_ld16(tmem_o + c0 + cc + lanes, o);
-                attn_ld_wait(o);
+              float top[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) o[k] *= rescale[c0 + cc + k];
-                attn_st16(tmem_o + c0 + cc + lanes, o);
-              }
+              for (int j = 0; j < 16; ++j) top[j] = cc < live ? x[cc + j] * cm : kNegInf;
+              warp_fold16<true>(top, lane);
+              if (!(lane & 1)) red[(tg * 4 + quarter) * kRows + c0 + cc + (lane >> 1)] = top[0];
             }
-            attn_st_wait();
-          }
-        }
-        // P, rounded, as the second product reads it (a score that is not seen is -inf, its P zero).
-        const uint32_t pt = smem_u32(p_s + (n % kNP) * Sh::kP);
+            bar_named(bar, kGroup);
+            if (gtid < kCols) {
+              const int col = c0 + gtid;
+              const float old = ref[col];
+              float now = old;
 #pragma unroll
-        for (int cc = 0; cc < kCols; cc += 8) {
-          if (cc < live) {
-            const float4 m0 = *reinterpret_cast<const float4*>(ref + c0 + cc), m1 = *reinterpret_cast<const float4*>(ref + c0 + cc + 4);
-            const float m[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
-            uint32_t w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              w[k] = pack16x2<kHalf>(ex2(fmaf(x[cc + 2 * k], cm, -m[2 * k])), ex2(fmaf(x[cc + 2 * k + 1], cm, -m[2 * k + 1])));
-              add16x2<kHalf>(w[k], l[cc + 2 * k], l[cc + 2 * k + 1]);
+              for (int w = 0; w < 4 * kTG; ++w) now = fmaxf(now, red[w * kRows + col]);
+              ref[col] = now;
+              rescale[col] = ex2(old - now);
             }
-            const int ch = (c0 + cc) >> 3;
-            uint32_t at;
-            if constexpr (kRows == 16) at = token * 32 + ((ch ^ ((token >> 2) & 1)) << 4);
-            else if constexpr (kRows == 32) at = token * 64 + ((ch ^ ((token >> 1) & 3)) << 4);
-            else at = (ch >> 3) * (kAttnTok * 128) + token * 128 + (((ch & 7) ^ (token & 7)) << 4);
-            st_shared_v4u(pt + at, w[0], w[1], w[2], w[3]);
-          }
-        }
-        if (group == 0) {
-          // V rows that not every row sees (see above). They are in the last tile or two of a request.
-          const bool ragged = (i + 1) * kAttnTok > s.r.kv, drafted = edge && s.r.drafted > 1;
-          if (ragged || drafted) {
-            ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax);
-            const uint32_t vt = smem_u32(ring_v + v_slot * Sh::kStage) + token * 128;
-            if (pos >= s.r.kv) {
+            bar_named(bar, kGroup);
+            if (i > s.i0) {
 #pragma unroll
-              for (int ch = 0; ch < kDim / 8; ++ch) st_shared_v4u(vt + (ch >> 3) * (kAttnTok * 128) + (ch & 7) * 16, 0u, 0u, 0u, 0u);
-            } else if (drafted && pos >= s.r.ctx) {
-              constexpr uint32_t kExp = kHalf ? 0x7C00u : 0x7F80u;
+              for (int j = 0; j < kCols; ++j)
+                if (j < live) l[j] *= rescale[c0 + j];
+              ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax);
+              tc_fence_after();
 #pragma unroll
-              for (int ch = 0; ch < kDim / 8; ++ch) {
-                const uint32_t at = vt + (ch >> 3) * (kAttnTok * 128) + (ch & 7) * 16;
-                const uint4 v = ld_shared_v4u(at);
-                uint32_t e[4] = {v.x, v.y, v.z, v.w};
-                bool odd = false;
+              for (int cc = 0; cc < kCols; cc += 16) {
+                if (cc < live && ((cc >> 4) & (kTG - 1)) == tg) {
+                  float o[16];
+                  attn_ld16(tmem_o + c0 + cc + lanes, o);
+                  attn_ld_wait(o);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  if ((e[k] & kExp) == kExp) e[k] &= 0xFFFF0000u, odd = true;
-                  if ((e[k] & (kExp << 16)) == (kExp << 16)) e[k] &= 0x0000FFFFu, odd = true;
-                }
-                if (odd) {
-                  st_shared_v4u(at, e[0], e[1], e[2], e[3]);
-                  *odd_v = 1;
+                  for (int k = 0; k < 16; ++k) o[k] *= rescale[c0 + cc + k];
+                  attn_st16(tmem_o + c0 + cc + lanes, o);
                 }
               }
+              attn_st_wait();
             }
           }
+          // P, rounded, as the second product reads it (a score that is not seen is -inf, its P zero).
+          const uint32_t pt = smem_u32(p_s + (n % kNP) * Sh::kP);
+#pragma unroll
+          for (int cc = 0; cc < kCols; cc += 8) {
+            if (cc < live) {
+              const float4 m0 = *reinterpret_cast<const float4*>(ref + c0 + cc), m1 = *reinterpret_cast<const float4*>(ref + c0 + cc + 4);
+              const float m[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+              uint32_t w[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                w[k] = pack16x2<kHalf>(ex2(fmaf(x[cc + 2 * k], cm, -m[2 * k])), ex2(fmaf(x[cc + 2 * k + 1], cm, -m[2 * k + 1])));
+                add16x2<kHalf>(w[k], l[cc + 2 * k], l[cc + 2 * k + 1]);
+              }
+              const int ch = (c0 + cc) >> 3;
+              uint32_t at;
+              if constexpr (kRows == 16) at = token * 32 + ((ch ^ ((token >> 2) & 1)) << 4);
+              else if constexpr (kRows == 32) at = token * 64 + ((ch ^ ((token >> 1) & 3)) << 4);
+              else at = (ch >> 3) * (kTok * 128) + token * 128 + (((ch & 7) ^ (token & 7)) << 4);
+              st_shared_v4u(pt + at, w[0], w[1], w[2], w[3]);
+            }
+          }
+          if (cg == 0) {
+            // V rows that not every row sees (see above). They are in the last tile or two of a request.
+            const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && s.r.drafted > 1;
+            if (ragged || drafted) {
+              ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax);
+              const uint32_t vt = smem_u32(ring_v + v_slot * Sh::kStage) + token * 128;
+              if (pos >= s.r.kv) {
+#pragma unroll
+                for (int ch = 0; ch < kDim / 8; ++ch) st_shared_v4u(vt + (ch >> 3) * (kTok * 128) + (ch & 7) * 16, 0u, 0u, 0u, 0u);
+              } else if (drafted && pos >= s.r.ctx) {
+                constexpr uint32_t kExp = kHalf ? 0x7C00u : 0x7F80u;
+#pragma unroll
+                for (int ch = 0; ch < kDim / 8; ++ch) {
+                  const uint32_t at = vt + (ch >> 3) * (kTok * 128) + (ch & 7) * 16;
+                  const uint4 v = ld_shared_v4u(at);
+                  uint32_t e[4] = {v.x, v.y, v.z, v.w};
+                  bool odd = false;
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    if ((e[k] & kExp) == kExp) e[k] &= 0xFFFF0000u, odd = true;
+                    if ((e[k] & (kExp << 16)) == (kExp << 16)) e[k] &= 0x0000FFFFu, odd = true;
+                  }
+                  if (odd) {
+                    st_shared_v4u(at, e[0], e[1], e[2], e[3]);
+                    *odd_v = 1;
+                  }
+                }
+              }
+            }
+          }
+          if (++v_slot == kNV) v_slot = 0, v_phase ^= 1u;
+          fence_proxy_async_shared();
+          tc_fence_before();
+          mbar_arrive(&p_full[n & 1u]);
         }
-        if (++v_slot == kNV) v_slot = 0, v_phase ^= 1u;
-        fence_proxy_async_shared();
-        tc_fence_before();
-        mbar_arrive(&p_full[n & 1u]);
-      }
-      ok = !bar_any(3, kAll, !ok);
-      if (!ok) break;
 
-      // ---- end of the segment: finish the row tile, or leave a partial -----------------------------
-      constexpr int kFold = kCols < 32 ? kCols : 32;
+        // ---- end of the segment: finish the row tile, or leave a partial ---------------------------
+        const bool whole = s.i0 == 0 && s.i1 == s.r.tiles;
 #pragma unroll
-      for (int cc = 0; cc < kCols; cc += kFold) {
-        warp_fold<kFold, false>(l + cc, lane);
-        if (kFold == 32 || !(lane & 1)) red[quarter * kRows + c0 + cc + (kFold == 32 ? lane : lane >> 1)] = l[cc];
-      }
-      bar_named(bar, 128);
-      const bool whole = s.i0 == 0 && s.i1 == s.r.tiles;
-      // The run that starts inside a row tile keeps its partial first, the one that ends inside it second.
-      const long long slot = (static_cast<long long>(blockIdx.x) * 2 + (s.i0 > 0 ? 0 : 1)) * kRows;
-      if (gtid < kCols) {
-        const int col = c0 + gtid;
-        const float sum = (red[col] + red[kRows + col]) + (red[2 * kRows + col] + red[3 * kRows + col]);
-        inv[col] = sum == 0.f ? 0.f : 1.f / sum;
-        if (!whole && col < rows) a.part_ml[slot + col] = make_float2(ref[col], sum);
-      }
-      ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax);
-      ok = !bar_any(3, kAll, !ok);
-      if (!ok) break;
-      tc_fence_after();
-      const int odd = *odd_v;
+        for (int cc = 0; cc < kCols; cc += 16) {
+          warp_fold16<false>(l + cc, lane);
+          if (!(lane & 1)) red[(tg * 4 + quarter) * kRows + c0 + cc + (lane >> 1)] = l[cc];
+        }
+        if (ok) ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax);
+        ok = !bar_any(8, kSoft, !ok);
+        if (!ok) break;
+        tc_fence_after();
+        // The run that starts inside a row tile keeps its partial first, the one that ends inside it second.
+        const int slot = (blockIdx.x * 2 + (s.i0 > 0 ? 0 : 1)) * kRows;
+        if (gtid < kCols) {
+          const int col = c0 + gtid;
+          float sum = 0.f;
 #pragma unroll
-      for (int cc = 0; cc < kCols; cc += 16) {
-        if (cc < live) {
-          float o[16];
-          attn_ld16(tmem_o + c0 + cc + lanes, o);
-          attn_ld_wait(o);
-          if (token < kDim) {
-            if (odd) {
-              // Put the non-finite entries back for the rows that see them.
-              const int j0 = max(s.i0 * kAttnTok - s.r.ctx, 0), j1 = min(min(s.i1 * kAttnTok, s.r.kv) - s.r.ctx, s.r.drafted);
-              for (int j = j0; j < j1; ++j) {
-                const int p = s.r.ctx + j;
-                const long long page = a.table[s.b * a.table_row + p / a.page];
-                if (page < 0 || page >= a.pages) continue;
-                const float v = lo16<kHalf>(a.v_pages[page * a.v_page + s.head * a.v_head + (p % a.page) * a.v_slot + token]);
-                if (!(fabsf(v) < __int_as_float(0x7f800000)))
+          for (int w = 0; w < 4 * kTG; ++w) sum += red[w * kRows + col];
+          inv[col] = sum == 0.f ? 0.f : 1.f / sum;
+          if (!whole && col < rows) a.part_ml[slot + col] = make_float2(ref[col], sum);
+        }
+        if (!whole && s.i0 == 0) {
+          cross.first = s.r.first, cross.row0 = s.row0, cross.rows = rows, cross.head = s.head;
+          cross.last = runs.of(s.unit0 + s.r.tiles - 1);
+        }
+        bar_named(bar, kGroup);
+        const int odd = *odd_v;
 #pragma unroll
-                  for (int k = 0; k < 16; ++k)
-                    if ((words[(c0 + cc + k) * 8 + (j >> 5)] >> (j & 31)) & 1u) o[k] += v;
+        for (int cc = 0; cc < kCols; cc += 16) {
+          if (cc < live && ((cc >> 4) & (kTG - 1)) == tg) {
+            float o[16];
+            attn_ld16(tmem_o + c0 + cc + lanes, o);
+            uint16_t gv[16];
+            const bool mine_o = tl < kDim;
+            if (whole && a.gate && mine_o) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) {
+                const int id = row_id[c0 + cc + k];
+                gv[k] = __ldg(a.gate + (s.r.first + (id >> 16)) * a.gate_token + (id & 0xFFFF) * a.gate_head + tl);
               }
             }
+            attn_ld_wait(o);
+            if (mine_o) {
+              if (odd) {
+                // Put the non-finite entries back for the rows that see them.
+                const int j0 = max(s.i0 * kTok - s.r.ctx, 0), j1 = min(min(s.i1 * kTok, s.r.kv) - s.r.ctx, s.r.drafted);
+                for (int j = j0; j < j1; ++j) {
+                  const int p = s.r.ctx + j;
+                  const long long page = a.table[s.b * a.table_row + p / a.page];
+                  if (page < 0 || page >= a.pages) continue;
+                  const float v = lo16<kHalf>(a.v_pages[page * a.v_page + s.head * a.v_head + (p % a.page) * a.v_slot + tl]);
+                  if (!(fabsf(v) < __int_as_float(0x7f800000)))
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const int col = c0 + cc + k;
-              if (col < rows) {
-                if (whole) {
-                  const int id = row_id[col], t = id >> 16, h = id & 0xFFFF;
-                  float v = o[k] * inv[col];
-                  if (a.gate) v /= 1.f + __expf(-lo16<kHalf>(a.gate[(s.r.first + t) * a.gate_token + h * a.gate_head + token]));
-                  a.out[(s.r.first + t) * a.out_token + h * a.out_head + token] =
-                      static_cast<uint16_t>(pack16x2<kHalf>(v, v) & 0xFFFFu);
-                } else {
-                  a.part_o[(slot + col) * kDim + token] = o[k];
+                    for (int k = 0; k < 16; ++k)
+                      if ((words[(c0 + cc + k) * 8 + (j >> 5)] >> (j & 31)) & 1u) o[k] += v;
                 }
+              }
+              if (whole) {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                  const int col = c0 + cc + k, id = row_id[col];
+                  float v = o[k] * inv[col];
+                  if (a.gate) v = __fdividef(v, 1.f + __expf(-lo16<kHalf>(gv[k])));
+                  if (col < rows)
+                    a.out[(s.r.first + (id >> 16)) * a.out_token + (id & 0xFFFF) * a.out_head + tl] =
+                        static_cast<uint16_t>(pack16x2<kHalf>(v, v) & 0xFFFFu);
+                }
+              } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k)
+                  if (c0 + cc + k < rows) a.part_o[static_cast<long long>(slot + c0 + cc + k) * kDim + tl] = o[k];
               }
             }
           }
         }
+        tc_fence_before();
       }
-      tc_fence_before();
     }
+    if (tid == 0) a.cross[blockIdx.x] = cross;
   }
   __syncthreads();
   if (warp == 1) {
@@ -736,83 +786,75 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   }
 }
 
-// Joins the partials of the row tiles that cross runs: one warp an output row. Weighs each partial by
-// 2^(its reference - the largest), in run order.
+// Joins the partials of the row tiles that cross runs: grid (runs, 16 parts of the rows), 8 warps, of which
+// each row has 128 / kRows (8 at 16 rows, 1 at 128) that take the runs in turn. Partials are weighed by
+// 2^(their reference - the largest) and added in a fixed order.
 template <bool kHalf, int kDim, int kRows>
-__global__ void __launch_bounds__(128) tree_attn_join_kernel(const AttnArgs a, int ctas) {
-  constexpr int kN = kDim / 32;
+__global__ void __launch_bounds__(256) tree_attn_join_kernel(const AttnArgs a) {
+  constexpr int kN = kDim / 32, kPerRow = 128 / kRows, kBlock = kRows / 16;
+  __shared__ float sums[8][kDim + 2];
   pdl_launch_dependents();
   pdl_wait();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long at = static_cast<long long>(blockIdx.x) * 4 + warp;
-  if (at >= static_cast<long long>(a.tokens) * a.heads) return;
-  const int t = static_cast<int>(at / a.heads), h = static_cast<int>(at % a.heads);
-  // The request with starts[b] <= t < starts[b + 1], 32 candidates a step.
-  int lo = 0, hi = a.requests;
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int cand = lo + lane * step;
-    const unsigned int below = __ballot_sync(0xffffffffu, cand < hi && a.starts[cand] <= t);
-    const int k = 31 - __clz(static_cast<int>(below | 1u));
-    lo += k * step;
-    hi = min(hi, lo + step);
-  }
-  const long long total = a.prefix[a.requests];
-  const AttnReq r = attn_request<kRows>(a, lo, false);
-  const int inner = t - r.first;
-  if (inner < 0 || inner >= r.drafted) return;
-  const int g = a.heads / a.kv_heads, head = h / g, row = inner * g + h - head * g;
-  const int row_tiles = (r.rows + kRows - 1) / kRows;
-  const long long w0 = a.prefix[lo] + (static_cast<long long>(head) * row_tiles + row / kRows) * r.tiles, w1 = w0 + r.tiles;
-  const int runs = attn_runs(total, ctas);
-  const int c0 = attn_run_of(total, w0, runs), c1 = attn_run_of(total, w1 - 1, runs);
-  if (c0 == c1) return;  // finished by its CTA
-  const int col = row % kRows;
-  auto slot = [&](int c) { return (static_cast<long long>(c) * 2 + (attn_run_start(total, c, runs) > w0 ? 0 : 1)) * kRows + col; };
+  const AttnCross x = a.cross[blockIdx.x];
+  const int r0 = blockIdx.y * kBlock;
+  if (r0 >= x.rows) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % kPerRow, col = r0 + warp / kPerRow;
+  const int c0 = blockIdx.x, n = x.last - c0 + 1;
+  const bool live = col < x.rows;
+  // Run c0 holds the tile's beginning in its second partial, the others their share in their first.
+  auto slot = [&](int k) { return static_cast<long long>((c0 + k) * 2 + (k == 0 ? 1 : 0)) * kRows + col; };
   float top = kAttnUnseen;
-  for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, a.part_ml[slot(c)].x);
+  if (live)
+    for (int k = lane; k < n; k += 32) top = fmaxf(top, a.part_ml[slot(k)].x);
 #pragma unroll
   for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   float acc[kN], sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kN; ++i) acc[i] = 0.f;
-  for (int c = c0; c <= c1; c += 32) {
-    float w = 0.f, part = 0.f;
-    long long mine = 0;
-    if (c + lane <= c1) {
-      mine = slot(c + lane);
-      const float2 ml = a.part_ml[mine];
-      w = ex2(ml.x - top);  // 0 for a partial that saw nothing beside one that saw something
-      part = ml.y * w;
-    }
-    const int n = min(32, c1 - c + 1);
+  if (live) {
 #pragma unroll 8
-    for (int k = 0; k < n; ++k) {
-      const float wk = __shfl_sync(0xffffffffu, w, k);
-      sum += __shfl_sync(0xffffffffu, part, k);
-      const float* src = a.part_o + __shfl_sync(0xffffffffu, mine, k) * kDim + lane * kN;
+    for (int k = part; k < n; k += kPerRow) {
+      const float2 ml = a.part_ml[slot(k)];
+      const float* src = a.part_o + slot(k) * kDim + lane * kN;
+      const float w = ex2(ml.x - top);  // 0 for a partial that saw nothing beside one that saw something
+      sum += ml.y * w;
       if constexpr (kN == 4) {
         const float4 v = *reinterpret_cast<const float4*>(src);
-        acc[0] += wk * v.x, acc[1] += wk * v.y, acc[2] += wk * v.z, acc[3] += wk * v.w;
+        acc[0] += w * v.x, acc[1] += w * v.y, acc[2] += w * v.z, acc[3] += w * v.w;
       } else {
         const float2 v = *reinterpret_cast<const float2*>(src);
-        acc[0] += wk * v.x, acc[1] += wk * v.y;
+        acc[0] += w * v.x, acc[1] += w * v.y;
       }
     }
   }
+  if constexpr (kPerRow > 1) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) sums[warp][lane * kN + i] = acc[i];
+    if (lane == 0) sums[warp][kDim] = sum;
+    __syncthreads();
+    if (part != 0) return;
+    for (int w = 1; w < kPerRow; ++w) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) acc[i] += sums[warp + w][lane * kN + i];
+      sum += sums[warp + w][kDim];
+    }
+  }
+  if (!live) return;
+  const int row = x.row0 + col, t = attn_token(a, row), g = a.heads / a.kv_heads;
+  const long long token = x.first + t, h = x.head * g + row - t * g;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint32_t packed[kN / 2];
 #pragma unroll
   for (int i = 0; i < kN; i += 2) {
     float v[2] = {acc[i] * inv, acc[i + 1] * inv};
     if (a.gate) {
-      const uint32_t gw = *reinterpret_cast<const uint32_t*>(a.gate + t * a.gate_token + h * a.gate_head + lane * kN + i);
-      v[0] /= 1.f + __expf(-lo16<kHalf>(gw));
-      v[1] /= 1.f + __expf(-hi16<kHalf>(gw));
+      const uint32_t gw = *reinterpret_cast<const uint32_t*>(a.gate + token * a.gate_token + h * a.gate_head + lane * kN + i);
+      v[0] = __fdividef(v[0], 1.f + __expf(-lo16<kHalf>(gw)));
+      v[1] = __fdividef(v[1], 1.f + __expf(-hi16<kHalf>(gw)));
     }
     packed[i / 2] = pack16x2<kHalf>(v[0], v[1]);
   }
-  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + t * a.out_token + h * a.out_head + lane * kN);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + token * a.out_token + h * a.out_head + lane * kN);
   if constexpr (kN == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);
   else dst[0] = packed[0];
 }
