@@ -6,6 +6,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <cstring>
 #include <atomic>
@@ -31,6 +32,7 @@
 #include "gemv_tiles.cuh"
 #include "rope_append.cuh"
 #include "tree_attn.cuh"
+#include "tree_attn_wide.cuh"
 #include "route.cuh"
 
 #define MUSE_VERSION_STRING "muse_proj_b200 0.1 (sm_100a)"

@@ -96,18 +96,19 @@ int check_attention(const MuseTreeAttention* p) {
   if (!p) return fail(MUSE_ERR_INVALID, "tree_attention: null arguments");
   if (int rc = check_heads("tree_attention", p->heads, p->kv_heads, p->dim, p->type)) return rc;
   if (p->tokens < 0 || p->requests < 0) return fail(MUSE_ERR_INVALID, "tree_attention: negative tokens or requests");
+  if (!std::isfinite(p->scale) || p->scale == 0.f) return fail(MUSE_ERR_INVALID, "tree_attention: scale must be finite and not 0");
   if (p->max_draft < 1 || p->max_draft > 256)
     return fail(MUSE_ERR_SHAPE, "tree_attention: max_draft must be 1..256 (got %d)", p->max_draft);
   return MUSE_OK;
 }
 
+// Rows of a unit: those that share a kv head, rounded up to a variant; past 64 the rows-as-M kernel's 256.
 int attention_rows(const MuseTreeAttention* p) {
-  // Rows that share a kv head, at most, rounded up to a row tile; past 128 several row tiles read the cache.
   const int64_t rows = static_cast<int64_t>(p->max_draft) * (p->heads / p->kv_heads);
-  return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 128));
+  return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 256));
 }
 
-int attention_tokens(int dim, int rows) {  // cached tokens a tile (AttnShape::kTok)
+int attention_tokens(int dim, int rows) {  // cached tokens a tile (AttnShape::kTok, WideShape::kTok)
   return dim == 64 && rows <= 32 ? 256 : 128;
 }
 
@@ -123,36 +124,43 @@ AttentionScratch attention_scratch(int rows, int dim, int ctas) {
   return s;
 }
 
-// 4-D map of one cache tensor: dims, entries of a page, kv heads, pages; boxes of 64 dims x `box` entries.
-int make_cache_map(CUtensorMap* map, const void* base, const MuseTreeAttention* p, int64_t page, int64_t head, int64_t entry, int box) {
+// 5-D map of one cache tensor: 64 dims, 8 entries, the halves of dim, groups of 8 entries in a page, and (page, kv head)
+// pairs as one coordinate, the head stride apart. A box is `entries` entries of one page and head, all of dim.
+int make_cache_map(CUtensorMap* map, const void* base, const MuseTreeAttention* p, int64_t head, int64_t entry, int64_t combo, int entries) {
   auto fn = encode_fn();
   if (!fn) return fail(MUSE_ERR_CUDA, "cuTensorMapEncodeTiled entry point not found");
-  cuuint64_t dims[4] = {static_cast<cuuint64_t>(p->dim), static_cast<cuuint64_t>(p->page_size), static_cast<cuuint64_t>(p->kv_heads),
-                        static_cast<cuuint64_t>(p->pages)};
-  cuuint64_t strides[3] = {static_cast<cuuint64_t>(entry * 2), static_cast<cuuint64_t>(head * 2), static_cast<cuuint64_t>(page * 2)};
-  cuuint32_t boxes[4] = {64u, static_cast<cuuint32_t>(box), 1u, 1u};
-  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
-  const CUresult r = fn(map, p->type == MUSE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+  const cuuint64_t pairs = static_cast<cuuint64_t>((p->pages - 1) * combo + p->kv_heads);
+  cuuint64_t dims[5] = {64, 8, static_cast<cuuint64_t>(p->dim / 64), static_cast<cuuint64_t>(p->page_size / 8), pairs};
+  cuuint64_t strides[4] = {static_cast<cuuint64_t>(entry * 2), 128, static_cast<cuuint64_t>(entry * 16), static_cast<cuuint64_t>(head * 2)};
+  cuuint32_t boxes[5] = {64u, 8u, static_cast<cuuint32_t>(p->dim / 64), static_cast<cuuint32_t>(entries / 8), 1u};
+  cuuint32_t estr[5] = {1u, 1u, 1u, 1u, 1u};
+  const CUresult r = fn(map, p->type == MUSE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
                         const_cast<void*>(base), dims, strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(MUSE_ERR_CUDA, "cuTensorMapEncodeTiled of the cache failed (%d)", static_cast<int>(r));
   return MUSE_OK;
 }
 
-template <bool kHalf, int kDim, int kRows>
-int launch_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas, cudaStream_t st) {
-  using Sh = muse::AttnShape<kDim, kRows>;
-  auto kern = muse::tree_attn_kernel<kHalf, kDim, kRows>;
+template <bool kHalf, int kDim, int kRows, typename Kern>
+int launch_attention_t(Kern kern, int threads, int smem, const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas,
+                       cudaStream_t st) {
   static bool configured[kMaxDevices] = {};
   int dev;
   if (int rc = current_device(&dev)) return rc;
   if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return fail(MUSE_ERR_CUDA, "cudaFuncSetAttribute(tree_attention): %s", cudaGetErrorString(e));
     configured[dev] = true;
   }
-  if (int rc = launch_pdl("tree_attention", kern, dim3(static_cast<unsigned>(ctas)), Sh::kThreads, Sh::kSmem, st, tmk, tmv, a)) return rc;
-  return launch_pdl("tree_attention join", muse::tree_attn_join_kernel<kHalf, kDim, kRows>, dim3(static_cast<unsigned>(ctas), 16), 256, 0, st, a);
+  if (int rc = launch_pdl("tree_attention", kern, dim3(static_cast<unsigned>(ctas)), threads, smem, st, tmk, tmv, a)) return rc;
+  return launch_pdl("tree_attention join", muse::tree_attn_join_kernel<kHalf, kDim, kRows>,
+                    dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(kRows / muse::attn_join_rows(kRows))), 256, 0, st, a);
+}
+
+template <bool kHalf, int kDim, int kRows>
+int launch_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas, cudaStream_t st) {
+  using Sh = muse::AttnShape<kDim, kRows>;
+  return launch_attention_t<kHalf, kDim, kRows>(muse::tree_attn_kernel<kHalf, kDim, kRows>, Sh::kThreads, Sh::kSmem, tmk, tmv, a, ctas, st);
 }
 
 template <bool kHalf, int kDim>
@@ -160,7 +168,8 @@ int launch_attention_rows(int rows, const CUtensorMap& tmk, const CUtensorMap& t
   if (rows == 16) return launch_attention<kHalf, kDim, 16>(tmk, tmv, a, ctas, st);
   if (rows == 32) return launch_attention<kHalf, kDim, 32>(tmk, tmv, a, ctas, st);
   if (rows == 64) return launch_attention<kHalf, kDim, 64>(tmk, tmv, a, ctas, st);
-  return launch_attention<kHalf, kDim, 128>(tmk, tmv, a, ctas, st);
+  using Sh = muse::WideShape<kDim>;
+  return launch_attention_t<kHalf, kDim, Sh::kRows>(muse::tree_attn_wide_kernel<kHalf, kDim>, Sh::kThreads, Sh::kSmem, tmk, tmv, a, ctas, st);
 }
 
 }  // namespace
@@ -200,7 +209,14 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   if (!aligned_to(p->table, 4) || !aligned_to(p->context, 4) || !aligned_to(p->starts, 4) || !aligned_to(p->mask, 4))
     return fail(MUSE_ERR_ALIGN, "tree_attention: table, context, starts and mask must be 4-byte aligned");
   for (int64_t x : {p->k_page, p->k_page_head, p->k_entry, p->v_page, p->v_page_head, p->v_entry})
-    if (x < 0 || x >= (int64_t(1) << 38)) return fail(MUSE_ERR_SHAPE, "tree_attention: cache strides must be 0..2^38 (got %lld)", (long long)x);
+    if (x < 1 || x >= (int64_t(1) << 35)) return fail(MUSE_ERR_SHAPE, "tree_attention: cache strides must be 1..2^35 (got %lld)", (long long)x);
+  // One kv head: the head stride is free, a page's takes its place.
+  const int64_t k_head = p->kv_heads == 1 ? p->k_page : p->k_page_head, v_head = p->kv_heads == 1 ? p->v_page : p->v_page_head;
+  const int64_t k_combo = p->pages == 1 ? p->kv_heads : p->k_page / k_head, v_combo = p->pages == 1 ? p->kv_heads : p->v_page / v_head;
+  if (p->pages > 1 && (p->k_page % k_head || p->v_page % v_head || k_combo < 1 || v_combo < 1))
+    return fail(MUSE_ERR_SHAPE, "tree_attention: the cache's page stride must be a multiple of its head stride");
+  if (p->pages > ((int64_t(1) << 31) - 1) / std::max(k_combo, v_combo) - 1)
+    return fail(MUSE_ERR_SHAPE, "tree_attention: the cache has too many pages (2^31 head strides)");
   DeviceInfo* d;
   if (int rc = device_info(&d)) return rc;
   const int tile = attention_rows(p);
@@ -210,8 +226,8 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   if (!aligned_to(p->scratch, 256)) return fail(MUSE_ERR_ALIGN, "tree_attention: scratch must be 256-byte aligned");
   const int box = std::min(p->page_size, attention_tokens(p->dim, tile));
   CUtensorMap tmk, tmv;
-  if (int rc = make_cache_map(&tmk, p->k_pages, p, p->k_page, p->k_page_head, p->k_entry, box)) return rc;
-  if (int rc = make_cache_map(&tmv, p->v_pages, p, p->v_page, p->v_page_head, p->v_entry, box)) return rc;
+  if (int rc = make_cache_map(&tmk, p->k_pages, p, k_head, p->k_entry, k_combo, box)) return rc;
+  if (int rc = make_cache_map(&tmv, p->v_pages, p, v_head, p->v_entry, v_combo, box)) return rc;
   muse::AttnArgs a;
   a.q = static_cast<const uint16_t*>(p->q);
   a.gate = static_cast<const uint16_t*>(p->gate);
@@ -226,7 +242,9 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   a.table_row = p->table_row, a.mask_row = p->mask_row, a.pages = p->pages;
   a.requests = p->requests, a.tokens = p->tokens, a.max_draft = p->max_draft, a.table_cols = p->table_cols;
   a.heads = p->heads, a.kv_heads = p->kv_heads, a.page = p->page_size;
-  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.scale_log2 = std::fabs(p->scale) * 1.4426950408889634f;
+  a.q_flip = p->scale < 0.f ? 0x80008000u : 0u;
+  a.k_combo = static_cast<int>(k_combo), a.v_combo = static_cast<int>(v_combo);
   a.mask_words = p->mask_words;
   const unsigned int group = static_cast<unsigned int>(p->heads / p->kv_heads);
   a.group_magic = group == 1 ? 0u : static_cast<unsigned int>(((uint64_t(1) << 32) + group - 1) / group);

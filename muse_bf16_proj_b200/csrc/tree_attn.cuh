@@ -7,7 +7,8 @@
 // is a stream of K and V tiles from HBM; the matrix products only have to keep up.
 //
 // Shape. The rows of a request that share a kv head (tokens x heads / kv_heads) are one operand, cut into row tiles of
-// kRows (16, 32, 64 or 128). Tokens are the tensor cores' M: a tile of 128 cached tokens gives
+// kRows (16, 32 or 64; more rows take the rows-as-M kernel of tree_attn_wide.cuh). Tokens are the tensor cores'
+// M: a tile of 128 cached tokens (two at dim 64 and up to 32 rows) gives
 //   S^T [128 tokens x kRows] = K [128 x dim] . Q^T        (UMMA M = 128, N = kRows; K as stored, K-major)
 //   O^T [dim x kRows]       += V^T [dim x 128] . P^T      (UMMA M = 128, N = kRows; V as stored, M-major)
 // so both operands from the cache enter as the TMA wrote them, few rows cost few columns (N = 16) instead of
@@ -57,8 +58,10 @@ struct AttnArgs {
   long long table_row, mask_row;
   long long pages;
   int requests, tokens, max_draft, table_cols, heads, kv_heads, page, mask_words;
+  int k_combo, v_combo;      // page stride / head stride: a (page, head) pair is one coordinate of the maps
   unsigned int group_magic;  // row / (heads / kv_heads) = umulhi(row, magic); 0: the group is one head
-  float scale_log2;          // scale * log2(e)
+  float scale_log2;          // |scale| * log2(e)
+  uint32_t q_flip;           // 0x80008000 where scale is negative: q is taken with the other sign
   struct AttnCross* cross;   // scratch: [ctas]
   float2* part_ml;           // scratch: [ctas][2][kRows] (reference maximum, sum)
   float* part_o;             // scratch: [ctas][2][kRows][dim]
@@ -89,8 +92,8 @@ struct AttnShape {
   static constexpr int kStage = kTok * kDim * 2;                  // one K or V tile
   static constexpr int kQ = kRows * kDim * 2;
   static constexpr int kP = kTok * kRows * 2;
-  static constexpr int kNP = kRows == 128 && kDim == 128 ? 1 : 2;  // P buffers
-  static constexpr int kNK = kDim == 64 ? (kRows <= 32 ? 3 : (kRows == 64 ? 5 : 4)) : (kRows <= 64 ? 3 : 2);
+  static constexpr int kNP = 2;                                   // P buffers
+  static constexpr int kNK = kDim == 64 && kRows == 64 ? 5 : 3;
   static constexpr int kNV = kDim == 64 ? (kRows == 32 ? 2 : kNK) : (kRows <= 32 ? 3 : 2);
   static constexpr int kTmemO = 2 * kTG * kRows;                  // after two buffers of S^T
   static constexpr int kTmem = kTmemO + kRows <= 64 ? 64 : (kTmemO + kRows <= 128 ? 128 : (kTmemO + kRows <= 256 ? 256 : 512));
@@ -183,12 +186,11 @@ struct AttnWalk {
   }
 };
 
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3,
-                                            uint64_t policy) {
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, uint64_t* bar, int c3, int c4, uint64_t policy) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(smem_u32(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %3, %3, %4, %5}], [%2], %6;" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(0), "r"(c3), "r"(c4), "l"(policy)
       : "memory");
 }
 
@@ -267,11 +269,161 @@ __device__ __forceinline__ void warp_fold16(float* v, int lane) {
   v[0] = kMax ? fmaxf(v[0], got) : v[0] + got;
 }
 
-// UMMA descriptor of an M- or N-major 16-bit operand: `row` bytes of M/N entries a k row (swizzled at that width),
-// groups of 8 k rows 8 * row apart, `chunk` bytes between runs of 64 M/N entries.
-__host__ __device__ constexpr uint64_t attn_mn_desc_bits(int row, int chunk) {
-  return (static_cast<uint64_t>(chunk >> 4) << 16) | (static_cast<uint64_t>((8 * row) >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+// UMMA descriptor but for its address: `row` bytes of a swizzled row, `group` bytes between groups of 8 rows,
+// `chunk` bytes between runs of 64 M/N entries (M- or N-major operands; 0: one run, or the same one again).
+__host__ __device__ constexpr uint64_t attn_desc_bits(int row, int group, int chunk) {
+  return (static_cast<uint64_t>(chunk >> 4) << 16) | (static_cast<uint64_t>(group >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
          (static_cast<uint64_t>(row == 128 ? 2 : (row == 64 ? 4 : 6)) << 61);
+}
+
+// The cached tokens of a tile in shared memory: groups of 8 tokens, each kHalves blocks (64 dims) of 8 rows of 128
+// bytes, swizzled within a block: what one TMA box {64 dims, 8 tokens, halves, groups} writes. A page's (or a
+// tile's) share is one box, its 2 * dim bytes a token contiguous in the cache as a rule.
+__device__ __forceinline__ uint32_t attn_row(int token, int halves) { return static_cast<uint32_t>((token >> 3) * 1024 * halves + (token & 7) * 128); }
+
+// Where a CTA's run starts: every CTA scans the requests (a run of requests a thread), none waits for another.
+struct AttnPlan {
+  AttnRuns runs;
+  int w0, w1, b0, s0;  // the run [w0, w1); its first request and the tiles before that
+  bool work;
+};
+template <int kThreads, int kTok, int kRows>
+__device__ __forceinline__ AttnPlan attn_plan(const AttnArgs& a, int* sums, int* start) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int total = 0, before = 0, mine = 0;
+  const int each = (a.requests + kThreads - 1) / kThreads;
+  const int b_lo = min(static_cast<int>(threadIdx.x) * each, a.requests), b_hi = min(b_lo + each, a.requests);
+  for (int b = b_lo; b < b_hi; ++b) {
+    const AttnReq r = attn_request<kTok, kRows>(a, b, blockIdx.x == 0);
+    mine += r.units * r.tiles;
+  }
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += x;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += sums[w];
+    total += sums[w];
+  }
+  before += upto - mine;
+  AttnPlan p = {AttnRuns(total, gridDim.x), 0, 0, 0, 0, false};
+  p.work = static_cast<int>(blockIdx.x) < p.runs.runs;
+  if (p.work) p.w0 = p.runs.start(blockIdx.x), p.w1 = p.runs.start(blockIdx.x + 1);
+  if (p.work && before <= p.w0 && p.w0 < before + mine) {
+    int at = before, b = b_lo;
+    if (each > 1) {
+      for (;; ++b) {
+        const AttnReq r = attn_request<kTok, kRows>(a, b, false);
+        if (p.w0 < at + r.units * r.tiles) break;
+        at += r.units * r.tiles;
+      }
+    }
+    start[0] = b, start[1] = at;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  p.b0 = start[0], p.s0 = start[1];
+  return p;
+}
+
+// The producer warp: K and V tiles of the run into their rings, a lane a box. Ends with no copy in flight.
+template <int kTok, int kRows, int kDim, int kNK, int kNV>
+__device__ __forceinline__ void attn_produce(const AttnArgs& a, const AttnPlan& plan, const CUtensorMap* tmk, const CUtensorMap* tmv,
+                                             uint8_t* ring_k, uint8_t* ring_v, uint64_t* k_full, uint64_t* k_empty, uint64_t* v_full,
+                                             uint64_t* v_empty) {
+  static_assert(kTok / 8 <= 32, "a lane a box");
+  constexpr int kStage = kTok * kDim * 2;
+  const int lane = threadIdx.x & 31;
+  int issued_k = 0, issued_v = 0;
+  AttnWalk<kTok, kRows> walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
+  AttnSeg s;
+  const int box = min(a.page, kTok), boxes = kTok / box;
+  const uint32_t off = static_cast<uint32_t>(lane * box * kDim * 2), box_bytes = static_cast<uint32_t>(box * kDim * 2);
+  // Tokens that several row tiles read stay in L2; a request's only reader streams them.
+  const uint64_t stream = policy_evict_first(), keep = policy_evict_normal();
+  Ring rk, rv;
+  bool ok = true;
+  while (ok && walk.next(a, s)) {
+    const uint64_t policy = s.r.rows > kRows ? keep : stream;
+    const int32_t* row = a.table + s.b * a.table_row;
+    int page = 0;
+    bool have = false;
+    auto lookup = [&](int i) {
+      const int pos = i * kTok + lane * box;
+      have = lane < boxes && pos < s.r.kv;
+      page = have ? row[static_cast<unsigned int>(pos) / static_cast<unsigned int>(a.page)] : 0;
+    };
+    lookup(s.i0);
+    for (int i = s.i0; i < s.i1; ++i) {
+      int now = page;
+      const int in = ((i * kTok + lane * box) & (a.page - 1)) >> 3;
+      const bool go = have;
+      if (go && (now < 0 || now >= a.pages)) report_error(kErrAttnPage), now = 0;
+      if (i + 1 < s.i1) lookup(i + 1);
+      const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, go))) * box_bytes;
+      ok = mbar_wait(&k_empty[rk.slot], rk.phase ^ 1u, kErrAttnProducer);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      if (lane == 0) mbar_expect_tx(&k_full[rk.slot], bytes);
+      __syncwarp();
+      if (go) tma_load_5d(ring_k + rk.slot * kStage + off, tmk, &k_full[rk.slot], in, now * a.k_combo + s.head, policy);
+      rk.next(kNK);
+      ++issued_k;
+      ok = mbar_wait(&v_empty[rv.slot], rv.phase ^ 1u, kErrAttnProducer);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      if (lane == 0) mbar_expect_tx(&v_full[rv.slot], bytes);
+      __syncwarp();
+      if (go) tma_load_5d(ring_v + rv.slot * kStage + off, tmv, &v_full[rv.slot], in, now * a.v_combo + s.head, policy);
+      rv.next(kNV);
+      ++issued_v;
+    }
+  }
+  for (int n = max(issued_k - kNK, 0); n < issued_k; ++n)
+    mbar_wait(&k_full[n % kNK], static_cast<uint32_t>((n / kNK) & 1), kErrAttnDrain, kWaitLimitNs / 100);
+  for (int n = max(issued_v - kNV, 0); n < issued_v; ++n)
+    mbar_wait(&v_full[n % kNV], static_cast<uint32_t>((n / kNV) & 1), kErrAttnDrain, kWaitLimitNs / 100);
+}
+
+// V rows that not every row of Q may see, before the second product reads them (0 x NaN is NaN): this thread's
+// token is zeroed past the request's end; a drafted one has non-finite entries zeroed and *odd set.
+template <bool kHalf, int kDim>
+__device__ __forceinline__ void attn_clean_v(uint32_t tile, int token, bool beyond, bool drafted, int* odd_v) {
+  constexpr int kHalves = kDim / 64;
+  const uint32_t row = tile + attn_row(token, kHalves);
+  if (beyond) {
+#pragma unroll
+    for (int ch = 0; ch < kDim / 8; ++ch) st_shared_v4u(row + (ch >> 3) * 1024 + (ch & 7) * 16, 0u, 0u, 0u, 0u);
+  } else if (drafted) {
+    constexpr uint32_t kExp = kHalf ? 0x7C00u : 0x7F80u;
+    for (int ch = 0; ch < kDim / 8; ++ch) {
+      const uint32_t at = row + (ch >> 3) * 1024 + (ch & 7) * 16;
+      const uint4 v = ld_shared_v4u(at);
+      uint32_t e[4] = {v.x, v.y, v.z, v.w};
+      bool odd = false;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if ((e[k] & kExp) == kExp) e[k] &= 0xFFFF0000u, odd = true;
+        if ((e[k] & (kExp << 16)) == (kExp << 16)) e[k] &= 0x0000FFFFu, odd = true;
+      }
+      if (odd) {
+        st_shared_v4u(at, e[0], e[1], e[2], e[3]);
+        *odd_v = 1;
+      }
+    }
+  }
+}
+
+// Word w of the drafted tokens that row `t` of request r sees: its mask's bits (or itself and every earlier token),
+// nothing past the request's tokens.
+__device__ __forceinline__ uint32_t attn_seen_word(const AttnArgs& a, const AttnReq& r, int t, int w) {
+  const uint32_t v = a.mask ? a.mask[(r.first + t) * a.mask_row + w] : 0xffffffffu;
+  const int n = (a.mask ? r.drafted : min(t + 1, r.drafted)) - w * 32;
+  return v & (n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u));
 }
 
 template <bool kHalf, int kDim, int kRows>
@@ -304,9 +456,8 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   uint64_t* pv_done = p_full + 2;
   uint64_t* q_full = pv_done + 2;
   uint64_t* fin = q_full + 1;
-  int* start_b = reinterpret_cast<int*>(fin + 1);  // the run's first request, and the tiles before it
-  int* start_s = start_b + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start_s + 1);
+  int* start_b = reinterpret_cast<int*>(fin + 1);  // [2]: the run's first request, and the tiles before it
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start_b + 2);
   int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);  // a drafted token of this segment has a non-finite V entry
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -324,132 +475,39 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
 
-  // Tiles before each request: a scan over the requests by the whole CTA, a run of requests a thread.
-  int total = 0, before = 0, mine = 0;
-  const int each = (a.requests + Sh::kThreads - 1) / Sh::kThreads;
-  const int b_lo = min(static_cast<int>(threadIdx.x) * each, a.requests), b_hi = min(b_lo + each, a.requests);
-  {
-    int* sums = reinterpret_cast<int*>(red);
-    int only = 0;
-    for (int b = b_lo; b < b_hi; ++b) {
-      const AttnReq r = attn_request<kTok, kRows>(a, b, blockIdx.x == 0);
-      only = r.units * r.tiles;
-      mine += only;
-    }
-    int upto = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += x;
-    }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < Sh::kThreads / 32; ++w) {
-      if (w < warp) before += sums[w];
-      total += sums[w];
-    }
-    before += upto - mine;
-  }
-  const AttnRuns runs(total, gridDim.x);
-  const bool work = static_cast<int>(blockIdx.x) < runs.runs;
-  const int w0 = work ? runs.start(blockIdx.x) : 0, w1 = work ? runs.start(blockIdx.x + 1) : 0;
-  if (work && before <= w0 && w0 < before + mine) {
-    int at = before, b = b_lo;
-    if (each > 1) {
-      for (;; ++b) {
-        const AttnReq r = attn_request<kTok, kRows>(a, b, false);
-        if (w0 < at + r.units * r.tiles) break;
-        at += r.units * r.tiles;
-      }
-    }
-    *start_s = at, *start_b = b;
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  const AttnPlan plan = attn_plan<Sh::kThreads, kTok, kRows>(a, reinterpret_cast<int*>(red), start_b);
   const uint32_t tmem = *tmem_slot;
-  const int b0 = *start_b, s0 = *start_s;
   const uint32_t tmem_o = tmem + Sh::kTmemO;
 
   if (warp == 0) {
-    // ---- producer: lane = one box ------------------------------------------------------------------
-    if (work) {
-      static_assert(kTok / 8 * kHalves <= 32, "a lane a box");
-      int issued_k = 0, issued_v = 0;
-      Walk walk(a, b0, s0, w0, w1);
-      AttnSeg s;
-      const int box = min(a.page, kTok), boxes = kTok / box;
-      const int half = lane / boxes, num = lane - half * boxes;  // 64-dim half and place of this lane's box
-      const uint32_t off = static_cast<uint32_t>(half * (kTok * 128) + num * box * 128);
-      // Tokens that several row tiles read stay in L2; a request's only reader streams them.
-      const uint64_t stream = policy_evict_first(), keep = policy_evict_normal();
-      Ring rk, rv;
-      bool ok = true;
-      while (ok && walk.next(a, s)) {
-        const uint64_t policy = s.r.rows > kRows ? keep : stream;
-        const int32_t* row = a.table + s.b * a.table_row;
-        int page = 0;
-        bool have = false;
-        auto lookup = [&](int i) {
-          const int pos = i * kTok + num * box;
-          have = half < kHalves && pos < s.r.kv;
-          page = have ? row[static_cast<unsigned int>(pos) / static_cast<unsigned int>(a.page)] : 0;
-        };
-        lookup(s.i0);
-        for (int i = s.i0; i < s.i1; ++i) {
-          const int now = page, in = (i * kTok + num * box) & (a.page - 1);
-          const bool go = have;
-          if (go && (now < 0 || now >= a.pages)) report_error(kErrAttnPage);  // reads as zeros: outside the map
-          if (i + 1 < s.i1) lookup(i + 1);
-          const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, go)) * box * 128);
-          ok = mbar_wait(&k_empty[rk.slot], rk.phase ^ 1u, kErrAttnProducer);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          if (lane == 0) mbar_expect_tx(&k_full[rk.slot], bytes);
-          __syncwarp();
-          if (go) tma_load_4d(ring_k + rk.slot * Sh::kStage + off, &tmk, &k_full[rk.slot], half * 64, in, s.head, now, policy);
-          rk.next(kNK);
-          ++issued_k;
-          ok = mbar_wait(&v_empty[rv.slot], rv.phase ^ 1u, kErrAttnProducer);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          if (lane == 0) mbar_expect_tx(&v_full[rv.slot], bytes);
-          __syncwarp();
-          if (go) tma_load_4d(ring_v + rv.slot * Sh::kStage + off, &tmv, &v_full[rv.slot], half * 64, in, s.head, now, policy);
-          rv.next(kNV);
-          ++issued_v;
-        }
-      }
-      // No copy may be in flight when the CTA ends, whichever way it does.
-      for (int n = max(issued_k - kNK, 0); n < issued_k; ++n)
-        mbar_wait(&k_full[n % kNK], static_cast<uint32_t>((n / kNK) & 1), kErrAttnDrain, kWaitLimitNs / 100);
-      for (int n = max(issued_v - kNV, 0); n < issued_v; ++n)
-        mbar_wait(&v_full[n % kNV], static_cast<uint32_t>((n / kNV) & 1), kErrAttnDrain, kWaitLimitNs / 100);
-    }
+    if (plan.work)
+      attn_produce<kTok, kRows, kDim, kNK, kNV>(a, plan, &tmk, &tmv, ring_k, ring_v, k_full, k_empty, v_full, v_empty);
   } else if (warp == 1) {
     // ---- UMMA issue --------------------------------------------------------------------------------
-    if (work && lane == 0) {
-      Walk walk(a, b0, s0, w0, w1);
+    if (plan.work && lane == 0) {
+      Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
       AttnSeg s;
       constexpr uint32_t kType = kHalf ? 0u : ((1u << 7) | (1u << 10));
       constexpr uint32_t kShape = (1u << 4) | (static_cast<uint32_t>(kRows >> 3) << 17) | (8u << 24);
       constexpr uint32_t idesc_s = kShape | kType, idesc_o = kShape | kType | (1u << 15) | (1u << 16);
       constexpr int kPRow = kRows >= 64 ? 128 : kRows * 2;  // bytes of a token's row of P
-      constexpr uint64_t v_bits = attn_mn_desc_bits(128, kDim == 128 ? kTok * 128 : 0);
-      constexpr uint64_t p_bits = attn_mn_desc_bits(kPRow, kRows == 128 ? kTok * 128 : 0);
+      constexpr uint64_t k_bits = attn_desc_bits(128, 1024 * kHalves, 16);
+      constexpr uint64_t v_bits = attn_desc_bits(128, 1024 * kHalves, kHalves > 1 ? 1024 : 0);
+      constexpr uint64_t p_bits = attn_desc_bits(kPRow, 8 * kPRow, 0);
       Ring rk, rv;
       uint32_t seg_phase = 0, n = 0;
       bool ok = true;
       auto issue_s = [&](uint32_t m) {
         if (!mbar_wait(&k_full[rk.slot], rk.phase, kErrAttnMma)) return false;
         tc_fence_after();
-        const uint64_t dk = umma_desc_sw128(smem_u32(ring_k + rk.slot * Sh::kStage)), dq = umma_desc_sw128(smem_u32(q_s));
+        const uint64_t dk = k_bits | ((smem_u32(ring_k + rk.slot * Sh::kStage) & 0x3FFFFu) >> 4), dq = umma_desc_sw128(smem_u32(q_s));
 #pragma unroll
         for (int t = 0; t < kTG; ++t)
 #pragma unroll
           for (int h = 0; h < kHalves; ++h)
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              umma_bf16(tmem + ((m & 1u) * kTG + t) * kRows, dk + ((h * kTok * 128 + t * 128 * 128) >> 4) + 2 * k,
+              umma_bf16(tmem + ((m & 1u) * kTG + t) * kRows, dk + ((h * 1024 + t * 128 * kDim * 2) >> 4) + 2 * k,
                         dq + ((h * kRows * 128) >> 4) + 2 * k, idesc_s, (h | k) != 0);
         umma_commit(&k_empty[rk.slot]);
         umma_commit(&s_full[m & 1u]);
@@ -472,7 +530,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           const uint64_t dp = p_bits | ((smem_u32(p_s + (n % kNP) * Sh::kP) & 0x3FFFFu) >> 4);
 #pragma unroll
           for (int k = 0; k < kTok / 16; ++k)
-            umma_bf16(tmem_o, dv + ((k * 16 * 128) >> 4), dp + ((k * 16 * kPRow) >> 4), idesc_o, (i > s.i0 || k > 0) ? 1u : 0u);
+            umma_bf16(tmem_o, dv + ((k * 16 * kDim * 2) >> 4), dp + ((k * 16 * kPRow) >> 4), idesc_o, (i > s.i0 || k > 0) ? 1u : 0u);
           umma_commit(&v_empty[rv.slot]);
           umma_commit(&pv_done[n & 1u]);
           rv.next(kNV);
@@ -496,8 +554,8 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     const float kNegInf = __int_as_float(0xff800000);
     const float c = a.scale_log2;
     AttnCross cross = {};
-    if (work) {
-      Walk walk(a, b0, s0, w0, w1);
+    if (plan.work) {
+      Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
       AttnSeg s;
       uint32_t n = 0;  // tiles done in this run
       uint32_t v_slot = 0, v_phase = 0;
@@ -521,19 +579,11 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
                                                          (s.head * g + s.row0 + r - t * g) * a.q_head + ch * 8));
           }
         }
-        // Drafted tokens that each row sees: bits up to itself without a mask; nothing past the request's tokens.
         const int nw = (s.r.drafted + 31) >> 5;
         for (int i = tid; i < full * 8; i += kSoft) {
           const int r = i >> 3, w = i & 7;
           if (w < nw) {
-            uint32_t v = 0u;
-            if (r < rows) {
-              const int t = attn_token(a, s.row0 + r);
-              v = a.mask ? a.mask[(s.r.first + t) * a.mask_row + w] : 0xffffffffu;
-              const int nb = (a.mask ? s.r.drafted : min(t + 1, s.r.drafted)) - w * 32;
-              v &= nb >= 32 ? 0xffffffffu : (nb <= 0 ? 0u : (1u << nb) - 1u);
-            }
-            words[i] = v;
+            words[i] = r < rows ? attn_seen_word(a, s.r, attn_token(a, s.row0 + r), w) : 0u;
           }
         }
         if (tid < kRows) {
@@ -546,8 +596,8 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         for (int u = 0; u < kLoads; ++u) {
           const int i = tid + u * kSoft, r = i / (kDim / 8), ch = i % (kDim / 8);
           if (r < full)
-            st_shared_v4u(smem_u32(q_s) + (ch >> 3) * (kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), qv[u].x, qv[u].y, qv[u].z,
-                          qv[u].w);
+            st_shared_v4u(smem_u32(q_s) + (ch >> 3) * (kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), qv[u].x ^ a.q_flip,
+                          qv[u].y ^ a.q_flip, qv[u].z ^ a.q_flip, qv[u].w ^ a.q_flip);
         }
         fence_proxy_async_shared();
         mbar_arrive(q_full);
@@ -557,8 +607,9 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         const bool lone = s.r.drafted == 1 && !a.mask;  // one token, which sees itself
 
         // ---- tiles ---------------------------------------------------------------------------------
-        for (int i = s.i0; ok && i < s.i1; ++i, ++n) {
-          ok = mbar_wait(&s_full[n & 1u], (n >> 1) & 1u, kErrAttnSoftmax);
+        // A wait that gave up is carried to the next barrier reduction: the loop's end has to be the same for all.
+        for (int i = s.i0; i < s.i1; ++i, ++n) {
+          ok = mbar_wait(&s_full[n & 1u], (n >> 1) & 1u, kErrAttnSoftmax) && ok;
           // P's buffer is free, and with two of them PV of two tiles ago is done, once this has passed.
           if (n >= static_cast<uint32_t>(kNP)) ok = mbar_wait(&pv_done[(n - kNP) & 1u], ((n - kNP) >> 1) & 1u, kErrAttnSoftmax) && ok;
           tc_fence_after();
@@ -586,17 +637,18 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
 #pragma unroll
             for (int k = 0; k < kCols; ++k) x[k] = (seen >> k) & 1u ? x[k] * c : kNegInf;
           }
-          bool past = false;
+          float over[4] = {kNegInf, kNegInf, kNegInf, kNegInf};  // how far a score passes its reference
 #pragma unroll
           for (int cc = 0; cc < kCols; cc += 4) {
             if (cc < live) {
               const float4 m = *reinterpret_cast<const float4*>(ref + c0 + cc);
-              past |= fmaf(x[cc], cm, -m.x) > kAttnSlack;
-              past |= fmaf(x[cc + 1], cm, -m.y) > kAttnSlack;
-              past |= fmaf(x[cc + 2], cm, -m.z) > kAttnSlack;
-              past |= fmaf(x[cc + 3], cm, -m.w) > kAttnSlack;
+              over[0] = fmaxf(over[0], fmaf(x[cc], cm, -m.x));
+              over[1] = fmaxf(over[1], fmaf(x[cc + 1], cm, -m.y));
+              over[2] = fmaxf(over[2], fmaf(x[cc + 2], cm, -m.z));
+              over[3] = fmaxf(over[3], fmaf(x[cc + 3], cm, -m.w));
             }
           }
+          const bool past = fmaxf(fmaxf(over[0], over[1]), fmaxf(over[2], over[3])) > kAttnSlack;
           if (bar_any(bar, kGroup, past || !ok)) {
             if (bar_any(bar, kGroup, !ok)) {
               ok = false;
@@ -626,7 +678,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
 #pragma unroll
               for (int j = 0; j < kCols; ++j)
                 if (j < live) l[j] *= rescale[c0 + j];
-              ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax);
+              ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax) && ok;
               tc_fence_after();
 #pragma unroll
               for (int cc = 0; cc < kCols; cc += 16) {
@@ -659,38 +711,16 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
               uint32_t at;
               if constexpr (kRows == 16) at = token * 32 + ((ch ^ ((token >> 2) & 1)) << 4);
               else if constexpr (kRows == 32) at = token * 64 + ((ch ^ ((token >> 1) & 3)) << 4);
-              else at = (ch >> 3) * (kTok * 128) + token * 128 + (((ch & 7) ^ (token & 7)) << 4);
+              else at = token * 128 + ((ch ^ (token & 7)) << 4);
               st_shared_v4u(pt + at, w[0], w[1], w[2], w[3]);
             }
           }
           if (cg == 0) {
-            // V rows that not every row sees (see above). They are in the last tile or two of a request.
+            // In the last tile or two of a request.
             const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && s.r.drafted > 1;
             if (ragged || drafted) {
-              ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax);
-              const uint32_t vt = smem_u32(ring_v + v_slot * Sh::kStage) + token * 128;
-              if (pos >= s.r.kv) {
-#pragma unroll
-                for (int ch = 0; ch < kDim / 8; ++ch) st_shared_v4u(vt + (ch >> 3) * (kTok * 128) + (ch & 7) * 16, 0u, 0u, 0u, 0u);
-              } else if (drafted && pos >= s.r.ctx) {
-                constexpr uint32_t kExp = kHalf ? 0x7C00u : 0x7F80u;
-#pragma unroll
-                for (int ch = 0; ch < kDim / 8; ++ch) {
-                  const uint32_t at = vt + (ch >> 3) * (kTok * 128) + (ch & 7) * 16;
-                  const uint4 v = ld_shared_v4u(at);
-                  uint32_t e[4] = {v.x, v.y, v.z, v.w};
-                  bool odd = false;
-#pragma unroll
-                  for (int k = 0; k < 4; ++k) {
-                    if ((e[k] & kExp) == kExp) e[k] &= 0xFFFF0000u, odd = true;
-                    if ((e[k] & (kExp << 16)) == (kExp << 16)) e[k] &= 0x0000FFFFu, odd = true;
-                  }
-                  if (odd) {
-                    st_shared_v4u(at, e[0], e[1], e[2], e[3]);
-                    *odd_v = 1;
-                  }
-                }
-              }
+              ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
+              attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), token, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);
             }
           }
           if (++v_slot == kNV) v_slot = 0, v_phase ^= 1u;
@@ -722,7 +752,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         }
         if (!whole && s.i0 == 0) {
           cross.first = s.r.first, cross.row0 = s.row0, cross.rows = rows, cross.head = s.head;
-          cross.last = runs.of(s.unit0 + s.r.tiles - 1);
+          cross.last = plan.runs.of(s.unit0 + s.r.tiles - 1);
         }
         bar_named(bar, kGroup);
         const int odd = *odd_v;
@@ -786,12 +816,14 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   }
 }
 
-// Joins the partials of the row tiles that cross runs: grid (runs, 16 parts of the rows), 8 warps, of which
-// each row has 128 / kRows (8 at 16 rows, 1 at 128) that take the runs in turn. Partials are weighed by
+__host__ __device__ constexpr int attn_join_rows(int rows) { return rows >= 128 ? 8 : rows / 16; }  // rows a CTA
+
+// Joins the partials of the row tiles that cross runs: grid (runs, parts of the rows), 8 warps, of which each
+// row has 8 (16 rows) to 1 (128 and more) that take the runs in turn. Partials are weighed by
 // 2^(their reference - the largest) and added in a fixed order.
 template <bool kHalf, int kDim, int kRows>
 __global__ void __launch_bounds__(256) tree_attn_join_kernel(const AttnArgs a) {
-  constexpr int kN = kDim / 32, kPerRow = 128 / kRows, kBlock = kRows / 16;
+  constexpr int kN = kDim / 32, kBlock = attn_join_rows(kRows), kPerRow = 8 / kBlock;
   __shared__ float sums[8][kDim + 2];
   pdl_launch_dependents();
   pdl_wait();

@@ -51,7 +51,9 @@ def test_rope_append_codes(change, code):
     (dict(table_cols=0), INVALID), (dict(dim=80), SHAPE), (dict(heads=5, kv_heads=2), SHAPE), (dict(max_draft=0), SHAPE),
     (dict(max_draft=257), SHAPE), (dict(page_size=4), SHAPE), (dict(page_size=24), SHAPE), (dict(page_size=2048), SHAPE),
     (dict(mask=16, mask_words=1, max_draft=33), SHAPE), (dict(q=24), ALIGN), (dict(q_token=60), ALIGN), (dict(v_entry=68), ALIGN),
-    (dict(gate=16, gate_token=4, gate_head=64), ALIGN), (dict(context=18), ALIGN)])
+    (dict(gate=16, gate_token=4, gate_head=64), ALIGN), (dict(context=18), ALIGN), (dict(scale=0.0), INVALID), (dict(scale=float("nan")), INVALID),
+    (dict(k_entry=0), SHAPE), (dict(v_page=1 << 40), SHAPE), (dict(kv_heads=2, heads=2, k_page=1544), SHAPE),
+    (dict(pages=1 << 31), SHAPE), (dict(table_cols=1 << 28), SHAPE), (dict(requests=1 << 20, table_cols=1 << 16), SHAPE)])
 def test_tree_attention_codes(change, code):
     assert _lib.load().muse_tree_attention(attention_args(**change), None) == code
     assert _lib.load().muse_last_error().startswith(b"tree_attention")
