@@ -391,6 +391,8 @@ __device__ __forceinline__ void attn_produce(const AttnArgs& a, const AttnPlan& 
 
 // V rows that not every row of Q may see, before the second product reads them (0 x NaN is NaN): this thread's
 // token is zeroed past the request's end; a drafted one has non-finite entries zeroed and *odd set.
+__device__ __forceinline__ uint4* attn_shared16(uint32_t addr) { return reinterpret_cast<uint4*>(__cvta_shared_to_generic(addr)); }
+
 template <bool kHalf, int kDim>
 __device__ __forceinline__ void attn_clean_v(uint32_t tile, int token, bool beyond, bool drafted, int* odd_v) {
   constexpr int kHalves = kDim / 64;
@@ -400,19 +402,24 @@ __device__ __forceinline__ void attn_clean_v(uint32_t tile, int token, bool beyo
     for (int ch = 0; ch < kDim / 8; ++ch) st_shared_v4u(row + (ch >> 3) * 1024 + (ch & 7) * 16, 0u, 0u, 0u, 0u);
   } else if (drafted) {
     constexpr uint32_t kExp = kHalf ? 0x7C00u : 0x7F80u;
-    for (int ch = 0; ch < kDim / 8; ++ch) {
-      const uint32_t at = row + (ch >> 3) * 1024 + (ch & 7) * 16;
-      const uint4 v = ld_shared_v4u(at);
-      uint32_t e[4] = {v.x, v.y, v.z, v.w};
-      bool odd = false;
+#pragma unroll 1
+    for (int c0 = 0; c0 < kDim / 8; c0 += 4) {
+      uint4 v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if ((e[k] & kExp) == kExp) e[k] &= 0xFFFF0000u, odd = true;
-        if ((e[k] & (kExp << 16)) == (kExp << 16)) e[k] &= 0x0000FFFFu, odd = true;
-      }
-      if (odd) {
-        st_shared_v4u(at, e[0], e[1], e[2], e[3]);
-        *odd_v = 1;
+      for (int u = 0; u < 4; ++u) v[u] = *attn_shared16(row + ((c0 + u) >> 3) * 1024 + ((c0 + u) & 7) * 16);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        uint32_t e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        bool odd = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if ((e[k] & kExp) == kExp) e[k] &= 0xFFFF0000u, odd = true;
+          if ((e[k] & (kExp << 16)) == (kExp << 16)) e[k] &= 0x0000FFFFu, odd = true;
+        }
+        if (odd) {
+          *attn_shared16(row + ((c0 + u) >> 3) * 1024 + ((c0 + u) & 7) * 16) = make_uint4(e[0], e[1], e[2], e[3]);
+          *odd_v = 1;
+        }
       }
     }
   }

@@ -17,6 +17,8 @@
 // References, partials, runs and entries that must not be seen are as in tree_attn.cuh.
 #pragma once
 
+#include <type_traits>
+
 #include "tree_attn.cuh"
 
 namespace muse {
@@ -37,15 +39,30 @@ struct WideShape {
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// 32 columns of this warp's lanes, not waited for, and the wait that the registers depend on.
-__device__ __forceinline__ void attn_ld32(uint32_t taddr, float (&v)[32]) {
-  attn_ld16(taddr, v);
-  attn_ld16(taddr + 16, v + 16);
+// kN columns of this warp's lanes.
+template <int kN>
+__device__ __forceinline__ void wide_ld(uint32_t taddr, float (&v)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN; i += 16) attn_ld16(taddr + i, v + i);
+#pragma unroll
+  for (int i = 0; i < kN; i += 16) attn_ld_wait(v + i);
 }
-__device__ __forceinline__ void attn_ld32_wait(float (&v)[32]) {
-  attn_ld_wait(v);
-  attn_ld_wait(v + 16);
+
+// Two FP32 fused multiply-adds (or sums) an instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
 }
+
+// 16 bytes from global to shared memory without a register; zeros where `live` is false.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // D (+)= A . B with A [128 x 16] in tensor memory (16-bit pairs), B from shared memory.
 __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
@@ -201,30 +218,17 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
         const bool pair = rows > 128;
         const int row = pair ? wg * 128 + tl : tl;                   // this thread's row of the unit
         const bool mine = row < rows;
-        const int t = mine ? attn_token(a, s.row0 + row) : 0, h = s.head * g + s.row0 + row - t * g;
+        const int t = mine ? attn_token(a, s.row0 + row) : 0;
         bar_named(8, 256);  // every thread is done with the last segment's arrays
-        // Q: each warp brings whole rows, 16 (8) lanes a row, eight loads in flight.
+        // Q: a thread a 16-byte chunk at a time, all of them on their way at once.
         const int q_rows = pair ? 256 : 128;
-        constexpr int kChunks = kDim / 8, kBatch = 8;
-        for (int base = 0; base < q_rows * kChunks; base += 256 * kBatch) {
-          uint4 qv[kBatch];
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const int i = base + tid + u * 256, r = i / kChunks, ch = i % kChunks;
-            qv[u] = make_uint4(0u, 0u, 0u, 0u);
-            if (r < rows) {
-              const int tr = attn_token(a, s.row0 + r);
-              qv[u] = __ldg(reinterpret_cast<const uint4*>(a.q + (s.r.first + tr) * a.q_token +
-                                                           (s.head * g + s.row0 + r - tr * g) * a.q_head + ch * 8));
-            }
-          }
-#pragma unroll
-          for (int u = 0; u < kBatch; ++u) {
-            const int i = base + tid + u * 256, r = i / kChunks, ch = i % kChunks;
-            if (r < q_rows)
-              st_shared_v4u(smem_u32(q_s) + (r >> 7) * Sh::kQ + (ch >> 3) * (128 * 128) + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4),
-                            qv[u].x ^ a.q_flip, qv[u].y ^ a.q_flip, qv[u].z ^ a.q_flip, qv[u].w ^ a.q_flip);
-          }
+        constexpr int kChunks = kDim / 8;
+        auto q_at = [&](int r, int ch) {
+          return smem_u32(q_s) + (r >> 7) * Sh::kQ + (ch >> 3) * (128 * 128) + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4);
+        };
+        for (int i = tid; i < q_rows * kChunks; i += 256) {
+          const int r = i / kChunks, ch = i % kChunks, rr = min(r, rows - 1), tr = attn_token(a, s.row0 + rr);
+          cp_async16(q_at(r, ch), a.q + (s.r.first + tr) * a.q_token + (s.head * g + s.row0 + rr - tr * g) * a.q_head + ch * 8, r < rows);
         }
         if (wg == 0 || pair) {
           const int nw = (s.r.drafted + 31) >> 5;
@@ -232,49 +236,53 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           for (int w = nw; w < 9; ++w) words[row * 9 + w] = 0u;
         }
         if (tid == 0) *odd_v = 0;
+        cp_async_wait();
+        if (a.q_flip) {  // a negative scale: this thread's own chunks with the other sign
+          for (int i = tid; i < q_rows * kChunks; i += 256) {
+            const uint32_t at = q_at(i / kChunks, i % kChunks);
+            const uint4 v = ld_shared_v4u(at);
+            st_shared_v4u(at, v.x ^ a.q_flip, v.y ^ a.q_flip, v.z ^ a.q_flip, v.w ^ a.q_flip);
+          }
+        }
         fence_proxy_async_shared();
         mbar_arrive(q_full);
         bar_named(8, 256);
 
-        // A thread's columns of a product, its products in the sequence, and its row's running values.
-        const int col0 = pair ? 0 : wg * 64, col1 = pair ? 128 : col0 + 64;
+        // The products of this thread's row tile in the sequence, and its row's running values.
         const int step = pair ? 2 : 1, products = (s.i1 - s.i0) << (pair ? 1 : 0);
         const uint32_t o_base = tmem_o + (pair ? wg * kDim : 0) + lanes;
         float ref = kAttnUnseen, l = 0.f;
-        // A wait that gave up is carried to the next vote: the loop's end has to be the same for a warp (pair) or all (lone).
-        for (int v = pair ? wg : 0; v < products; v += step) {
+        // One product's softmax over this thread's kN columns (128: pair, 64: lone). False: a wait gave up, for all
+        // threads that share a vote (a warp, or both warpgroups).
+        auto product = [&](auto columns, int v) {
+          constexpr int kN = decltype(columns)::value;
+          constexpr bool kPair = kN == 128;
           const uint32_t n = v0 + v, buffer = n & 1u;
-          const int i = s.i0 + (pair ? v >> 1 : v);
+          const int i = s.i0 + (kPair ? v >> 1 : v), col0 = kPair ? 0 : wg * 64;
           ok = mbar_wait(&s_full[buffer], (n >> 1) & 1u, kErrAttnSoftmax) && ok;
           tc_fence_after();
           const uint32_t ts = tmem + buffer * 128 + lanes;
+          float x[kN];
+          wide_ld<kN>(ts + col0, x);
           const bool edge = (i + 1) * kTok > s.r.ctx;  // the tile reaches past the context
-          // Largest score of the row (of this thread's columns).
-          float top = kNegInf;
-          for (int cc = col0; cc < col1; cc += 32) {
-            float x[32];
-            attn_ld32(ts + cc, x);
-            attn_ld32_wait(x);
-            if (edge) {
-              const uint32_t seen = wide_seen(words + row * 9, i * kTok + cc - s.r.ctx);
+          if (edge) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = (seen >> k) & 1u ? x[k] : kNegInf;
+            for (int cc = 0; cc < kN; cc += 32) {
+              const uint32_t seen = wide_seen(words + row * 9, i * kTok + col0 + cc - s.r.ctx);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) x[cc + k] = (seen >> k) & 1u ? x[cc + k] : kNegInf;
             }
-            float m[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-            for (int k = 4; k < 32; ++k) m[k & 3] = fmaxf(m[k & 3], x[k]);
-            top = fmaxf(top, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
           }
-          top *= c;
-          const bool past = top - ref > kAttnSlack;
-          // Whether this warp (pair) or the CTA's softmax threads (lone) have a reference to move.
-          const bool move = pair ? __any_sync(0xffffffffu, past || !ok) : bar_any(8, 256, past || !ok);
-          if (move) {
-            if (pair ? __any_sync(0xffffffffu, !ok) : bar_any(8, 256, !ok)) {
-              ok = false;
-              break;
-            }
-            if (!pair) {
+          float m[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int k = 4; k < kN; ++k) m[k & 3] = fmaxf(m[k & 3], x[k]);
+          float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c;
+          // Whether this warp (pair) or any softmax thread (lone; S has been read by both warpgroups after this) has a
+          // reference to move.
+          const bool past = top - ref > kAttnSlack || !ok;
+          if (kPair ? __any_sync(0xffffffffu, past) : bar_any(8, 256, past)) {
+            if (kPair ? __any_sync(0xffffffffu, !ok) : bar_any(8, 256, !ok)) return false;
+            if (!kPair) {
               swap[wg * 128 + tl] = top;
               bar_named(8, 256);
               top = fmaxf(top, swap[(wg ^ 1) * 128 + tl]);
@@ -285,55 +293,38 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
             l *= f;
             if (v >= step) {
               // O is whole up to the product before: the pair's last of this row tile came before S, the lone one's not.
-              if (!pair) {
+              if (!kPair) {
                 ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax) && ok;
                 tc_fence_after();
               }
-              const int d0 = pair ? 0 : wg * (kDim / 2), d1 = pair ? kDim : d0 + kDim / 2;
-              for (int d = d0; d < d1; d += 32) {
-                float o[32];
-                attn_ld32(o_base + d, o);
-                attn_ld32_wait(o);
+              const int d0 = kPair ? 0 : wg * (kDim / 2), d1 = kPair ? kDim : d0 + kDim / 2;
+#pragma unroll 1
+              for (int d = d0; d < d1; d += 16) {
+                float o[16];
+                wide_ld<16>(o_base + d, o);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] *= f;
+                for (int k = 0; k < 16; ++k) o[k] *= f;
                 attn_st16(o_base + d, o);
-                attn_st16(o_base + d + 16, o + 16);
               }
               attn_st_wait();
             }
           }
-          // P over S's columns, rounded; 32 scores become 16 words, behind what is still to be read. (Lone: the
-          // second warpgroup writes over columns the first may still have to read, so it waits for it below.)
-          uint32_t w[2][16];
-          for (int cc = col0; cc < col1; cc += 32) {
-            float x[32];
-            attn_ld32(ts + cc, x);
-            attn_ld32_wait(x);
-            if (edge) {
-              const uint32_t seen = wide_seen(words + row * 9, i * kTok + cc - s.r.ctx);
+          // P, rounded, over S's columns: 32 scores become 16 words.
+          float2 sum = {0.f, 0.f};
+          const float2 cc2 = {c, c}, mm2 = {-ref, -ref};
 #pragma unroll
-              for (int k = 0; k < 32; ++k) x[k] = (seen >> k) & 1u ? x[k] : kNegInf;
-            }
-            float l0 = 0.f, l1 = 0.f;
-            uint32_t p[16];
+          for (int cc = 0; cc < kN; cc += 32) {
+            float p[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              p[k] = pack16x2<kHalf>(ex2(fmaf(x[2 * k], c, -ref)), ex2(fmaf(x[2 * k + 1], c, -ref)));
-              add16x2<kHalf>(p[k], l0, l1);
+              const float2 e = fma2({x[cc + 2 * k], x[cc + 2 * k + 1]}, cc2, mm2);
+              const uint32_t w = pack16x2<kHalf>(ex2(e.x), ex2(e.y));
+              add16x2<kHalf>(w, sum.x, sum.y);
+              p[k] = __uint_as_float(w);
             }
-            l += l0 + l1;
-            if (pair) {
-              attn_st16(ts + (cc >> 1), reinterpret_cast<const float*>(p));
-            } else {
-#pragma unroll
-              for (int k = 0; k < 16; ++k) w[0][k] = cc == col0 ? p[k] : w[0][k], w[1][k] = p[k];
-            }
+            attn_st16(ts + ((col0 + cc) >> 1), p);
           }
-          if (!pair) {
-            bar_named(8, 256);  // both warpgroups have read all of S
-            attn_st16(ts + (col0 >> 1), reinterpret_cast<const float*>(w[0]));
-            attn_st16(ts + (col0 >> 1) + 16, reinterpret_cast<const float*>(w[1]));
-          }
+          l += sum.x + sum.y;
           attn_st_wait();
           if (wg == 0) {
             const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && s.r.drafted > 1;
@@ -346,8 +337,17 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           }
           if (++v_slot == kNV) v_slot = 0, v_phase ^= 1u;
           tc_fence_before();
-          if (pair) mbar_arrive_n(&p_full[buffer], 2);
+          if (kPair) mbar_arrive_n(&p_full[buffer], 2);
           else mbar_arrive(&p_full[buffer]);
+          return true;
+        };
+        // A wait that gave up is carried to the next vote: the loop's end has to be the same for all that vote.
+        if (pair) {
+          for (int v = wg; v < products; v += 2)
+            if (!product(std::integral_constant<int, 128>{}, v)) break;
+        } else {
+          for (int v = 0; v < products; ++v)
+            if (!product(std::integral_constant<int, 64>{}, v)) break;
         }
 
         // ---- end of the segment: finish the rows, or leave a partial ---------------------------------
@@ -368,56 +368,63 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           cross.first = s.r.first, cross.row0 = s.row0, cross.rows = rows, cross.head = s.head;
           cross.last = plan.runs.of(s.unit0 + s.r.tiles - 1);
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);
         const int odd = *odd_v;
-        const int d0 = pair ? 0 : wg * (kDim / 2), d1 = pair ? kDim : d0 + kDim / 2;
-        for (int d = d0; d < d1; d += 32) {
-          float o[32];
-          attn_ld32(o_base + d, o);
-          uint4 gv[4];
-          if (whole && a.gate && mine) {
-            const uint4* src = reinterpret_cast<const uint4*>(a.gate + (s.r.first + t) * a.gate_token + h * a.gate_head + d);
+        // Rows leave through Q's place (its products are done), half of dim at a time: [128 rows][kDim / 2] FP32 a
+        // warpgroup, 16-byte chunks swizzled by the row, so that a warp writes whole lines.
+        constexpr int kPart = kDim / 2, kPieces = kPart / 4;
+        const uint32_t stage = smem_u32(q_s) + wg * Sh::kQ;
+        for (int d = pair ? 0 : wg * kPart; d < (pair ? kDim : (wg + 1) * kPart); d += kPart) {
+          bar_named(1 + wg, 128);
+#pragma unroll 1
+          for (int e = 0; e < kPart; e += 16) {
+            float o[16];
+            wide_ld<16>(o_base + d + e, o);
+            if (odd && mine) {
+              // Put the non-finite entries back for the rows that see them.
+              const int j0 = max(s.i0 * kTok - s.r.ctx, 0), j1 = min(min(s.i1 * kTok, s.r.kv) - s.r.ctx, s.r.drafted);
+              for (int j = j0; j < j1; ++j) {
+                if (!((words[row * 9 + (j >> 5)] >> (j & 31)) & 1u)) continue;
+                const int p = s.r.ctx + j;
+                const long long page = a.table[s.b * a.table_row + p / a.page];
+                if (page < 0 || page >= a.pages) continue;
+                const uint16_t* src = a.v_pages + page * a.v_page + s.head * a.v_head + (p % a.page) * a.v_slot + d + e;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) gv[k] = __ldg(src + k);
-          }
-          attn_ld32_wait(o);
-          if (!mine) continue;
-          if (odd) {
-            // Put the non-finite entries back for the rows that see them.
-            const int j0 = max(s.i0 * kTok - s.r.ctx, 0), j1 = min(min(s.i1 * kTok, s.r.kv) - s.r.ctx, s.r.drafted);
-            for (int j = j0; j < j1; ++j) {
-              if (!((words[row * 9 + (j >> 5)] >> (j & 31)) & 1u)) continue;
-              const int p = s.r.ctx + j;
-              const long long page = a.table[s.b * a.table_row + p / a.page];
-              if (page < 0 || page >= a.pages) continue;
-              const uint16_t* src = a.v_pages + page * a.v_page + s.head * a.v_head + (p % a.page) * a.v_slot + d;
-#pragma unroll
-              for (int k = 0; k < 32; ++k) {
-                const float e = lo16<kHalf>(src[k]);
-                if (!(fabsf(e) < __int_as_float(0x7f800000))) o[k] += e;
+                for (int k = 0; k < 16; ++k) {
+                  const float x = lo16<kHalf>(src[k]);
+                  if (!(fabsf(x) < __int_as_float(0x7f800000))) o[k] += x;
+                }
               }
             }
-          }
-          if (whole) {
-            uint32_t p[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float e0 = o[2 * k] * inv, e1 = o[2 * k + 1] * inv;
+            for (int k = 0; k < 16; k += 4) {
+              const int ch = (e + k) >> 2;
+              st_shared_v4u(stage + tl * (kPart * 4) + ((ch ^ (tl & (kPieces - 1))) << 4), __float_as_uint(o[k] * inv),
+                            __float_as_uint(o[k + 1] * inv), __float_as_uint(o[k + 2] * inv), __float_as_uint(o[k + 3] * inv));
+            }
+          }
+          bar_named(1 + wg, 128);
+          const int first = pair ? wg * 128 : 0;  // the unit's row of this warpgroup's row 0
+          for (int u = tid & 127; u < 128 * kPieces; u += 128) {
+            const int r = u / kPieces, ch = u % kPieces, of = first + r;
+            if (of >= rows) break;  // rows ascend with u
+            const float4 o = ld_shared_v4(stage + r * (kPart * 4) + ((ch ^ (r & (kPieces - 1))) << 4));
+            if (whole) {
+              const int tr = attn_token(a, s.row0 + of), hr = s.head * g + s.row0 + of - tr * g;
+              float e[4] = {o.x, o.y, o.z, o.w};
               if (a.gate) {
-                const uint4 q4 = gv[k >> 2];
-                const uint32_t gw = (k & 3) == 0 ? q4.x : ((k & 3) == 1 ? q4.y : ((k & 3) == 2 ? q4.z : q4.w));
-                e0 = __fdividef(e0, 1.f + __expf(-lo16<kHalf>(gw)));
-                e1 = __fdividef(e1, 1.f + __expf(-hi16<kHalf>(gw)));
+                const uint2 gw = __ldg(reinterpret_cast<const uint2*>(a.gate + (s.r.first + tr) * a.gate_token + hr * a.gate_head + d + ch * 4));
+                e[0] = __fdividef(e[0], 1.f + __expf(-lo16<kHalf>(gw.x)));
+                e[1] = __fdividef(e[1], 1.f + __expf(-hi16<kHalf>(gw.x)));
+                e[2] = __fdividef(e[2], 1.f + __expf(-lo16<kHalf>(gw.y)));
+                e[3] = __fdividef(e[3], 1.f + __expf(-hi16<kHalf>(gw.y)));
               }
-              p[k] = pack16x2<kHalf>(e0, e1);
+              *reinterpret_cast<uint2*>(a.out + (s.r.first + tr) * a.out_token + hr * a.out_head + d + ch * 4) =
+                  make_uint2(pack16x2<kHalf>(e[0], e[1]), pack16x2<kHalf>(e[2], e[3]));
+            } else {
+              const long long at = (static_cast<long long>(blockIdx.x) * 2 + (s.i0 > 0 ? 0 : 1)) * Sh::kRows + of;
+              *reinterpret_cast<float4*>(a.part_o + at * kDim + d + ch * 4) = o;
             }
-            uint4* dst = reinterpret_cast<uint4*>(a.out + (s.r.first + t) * a.out_token + h * a.out_head + d);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) dst[k] = make_uint4(p[4 * k], p[4 * k + 1], p[4 * k + 2], p[4 * k + 3]);
-          } else {
-            float4* dst = reinterpret_cast<float4*>(a.part_o + slot * kDim + d);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
         }
         tc_fence_before();
