@@ -230,6 +230,16 @@ __device__ __forceinline__ bool bar_any(int id, int threads, bool p) {
   return r != 0u;
 }
 
+// One lane of a converged warp. The UMMA warp runs its loop with all lanes, on values made uniform with a
+// shuffle, and elects a lane around the tcgen05 instructions alone: descriptors then live in uniform registers. With
+// the whole loop under `lane == 0` each UMMA took about 105 cycles to issue, more than the 64 an N = 128 one runs for.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0u;
+}
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -402,24 +412,30 @@ __device__ __forceinline__ void attn_clean_v(uint32_t tile, int token, bool beyo
     for (int ch = 0; ch < kDim / 8; ++ch) st_shared_v4u(row + (ch >> 3) * 1024 + (ch & 7) * 16, 0u, 0u, 0u, 0u);
   } else if (drafted) {
     constexpr uint32_t kExp = kHalf ? 0x7C00u : 0x7F80u;
+    constexpr uint32_t kBit = kHalf ? 0x04000400u : 0x00800080u;  // an exponent of all ones carries into the sign's place
 #pragma unroll 1
     for (int c0 = 0; c0 < kDim / 8; c0 += 4) {
       uint4 v[4];
+      uint32_t any = 0u;
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = *attn_shared16(row + ((c0 + u) >> 3) * 1024 + ((c0 + u) & 7) * 16);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
+        const uint32_t e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any |= (e[k] & (kExp * 0x10001u)) + kBit;
+      }
+      if (!(any & 0x80008000u)) continue;
+      *odd_v = 1;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
         uint32_t e[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-        bool odd = false;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          if ((e[k] & kExp) == kExp) e[k] &= 0xFFFF0000u, odd = true;
-          if ((e[k] & (kExp << 16)) == (kExp << 16)) e[k] &= 0x0000FFFFu, odd = true;
+          if ((e[k] & kExp) == kExp) e[k] &= 0xFFFF0000u;
+          if ((e[k] & (kExp << 16)) == (kExp << 16)) e[k] &= 0x0000FFFFu;
         }
-        if (odd) {
-          *attn_shared16(row + ((c0 + u) >> 3) * 1024 + ((c0 + u) & 7) * 16) = make_uint4(e[0], e[1], e[2], e[3]);
-          *odd_v = 1;
-        }
+        *attn_shared16(row + ((c0 + u) >> 3) * 1024 + ((c0 + u) & 7) * 16) = make_uint4(e[0], e[1], e[2], e[3]);
       }
     }
   }
@@ -467,7 +483,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start_b + 2);
   int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);  // a drafted token of this segment has a non-finite V entry
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tmk);
     prefetch_tensormap(&tmv);
@@ -483,7 +499,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   pdl_wait();
 
   const AttnPlan plan = attn_plan<Sh::kThreads, kTok, kRows>(a, reinterpret_cast<int*>(red), start_b);
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(*tmem_slot)));
   const uint32_t tmem_o = tmem + Sh::kTmemO;
 
   if (warp == 0) {
@@ -491,7 +507,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       attn_produce<kTok, kRows, kDim, kNK, kNV>(a, plan, &tmk, &tmv, ring_k, ring_v, k_full, k_empty, v_full, v_empty);
   } else if (warp == 1) {
     // ---- UMMA issue --------------------------------------------------------------------------------
-    if (plan.work && lane == 0) {
+    if (uniform(plan.work)) {
       Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
       AttnSeg s;
       constexpr uint32_t kType = kHalf ? 0u : ((1u << 7) | (1u << 10));
@@ -504,46 +520,55 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       Ring rk, rv;
       uint32_t seg_phase = 0, n = 0;
       bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrAttnMma)) != 0; };
       auto issue_s = [&](uint32_t m) {
-        if (!mbar_wait(&k_full[rk.slot], rk.phase, kErrAttnMma)) return false;
+        if (!wait(&k_full[rk.slot], rk.phase)) return false;
         tc_fence_after();
-        const uint64_t dk = k_bits | ((smem_u32(ring_k + rk.slot * Sh::kStage) & 0x3FFFFu) >> 4), dq = umma_desc_sw128(smem_u32(q_s));
+        if (elect_one()) {
+          const uint64_t dk = k_bits | ((smem_u32(ring_k + rk.slot * Sh::kStage) & 0x3FFFFu) >> 4), dq = umma_desc_sw128(smem_u32(q_s));
 #pragma unroll
-        for (int t = 0; t < kTG; ++t)
+          for (int t = 0; t < kTG; ++t)
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h)
+            for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_bf16(tmem + ((m & 1u) * kTG + t) * kRows, dk + ((h * 1024 + t * 128 * kDim * 2) >> 4) + 2 * k,
-                        dq + ((h * kRows * 128) >> 4) + 2 * k, idesc_s, (h | k) != 0);
-        umma_commit(&k_empty[rk.slot]);
-        umma_commit(&s_full[m & 1u]);
+              for (int k = 0; k < 4; ++k)
+                umma_bf16(tmem + ((m & 1u) * kTG + t) * kRows, dk + ((h * 1024 + t * 128 * kDim * 2) >> 4) + 2 * k,
+                          dq + ((h * kRows * 128) >> 4) + 2 * k, idesc_s, (h | k) != 0);
+          umma_commit(&k_empty[rk.slot]);
+          umma_commit(&s_full[m & 1u]);
+        }
+        __syncwarp();
         rk.next(kNK);
         return true;
       };
-      while (ok && walk.next(a, s)) {
-        ok = mbar_wait(q_full, seg_phase, kErrAttnMma);
+      while (ok && uniform(walk.next(a, s))) {
+        const int tiles = uniform(s.i1 - s.i0);
+        ok = wait(q_full, seg_phase);
         seg_phase ^= 1u;
         if (!ok) break;
         tc_fence_after();
         ok = issue_s(n);
-        for (int i = s.i0; ok && i < s.i1; ++i, ++n) {
+        for (int i = 0; ok && i < tiles; ++i, ++n) {
           // The next tile's scores are under way while the softmax of this one runs.
-          if (i + 1 < s.i1 && !(ok = issue_s(n + 1))) break;
-          ok = mbar_wait(&p_full[n & 1u], (n >> 1) & 1u, kErrAttnMma) && mbar_wait(&v_full[rv.slot], rv.phase, kErrAttnMma);
+          if (i + 1 < tiles && !(ok = issue_s(n + 1))) break;
+          ok = wait(&p_full[n & 1u], (n >> 1) & 1u) && wait(&v_full[rv.slot], rv.phase);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t dv = v_bits | ((smem_u32(ring_v + rv.slot * Sh::kStage) & 0x3FFFFu) >> 4);
-          const uint64_t dp = p_bits | ((smem_u32(p_s + (n % kNP) * Sh::kP) & 0x3FFFFu) >> 4);
+          if (elect_one()) {
+            const uint64_t dv = v_bits | ((smem_u32(ring_v + rv.slot * Sh::kStage) & 0x3FFFFu) >> 4);
+            const uint64_t dp = p_bits | ((smem_u32(p_s + (n % kNP) * Sh::kP) & 0x3FFFFu) >> 4);
 #pragma unroll
-          for (int k = 0; k < kTok / 16; ++k)
-            umma_bf16(tmem_o, dv + ((k * 16 * kDim * 2) >> 4), dp + ((k * 16 * kPRow) >> 4), idesc_o, (i > s.i0 || k > 0) ? 1u : 0u);
-          umma_commit(&v_empty[rv.slot]);
-          umma_commit(&pv_done[n & 1u]);
+            for (int k = 0; k < kTok / 16; ++k)
+              umma_bf16(tmem_o, dv + ((k * 16 * kDim * 2) >> 4), dp + ((k * 16 * kPRow) >> 4), idesc_o, (i > 0 || k > 0) ? 1u : 0u);
+            umma_commit(&v_empty[rv.slot]);
+            umma_commit(&pv_done[n & 1u]);
+          }
+          __syncwarp();
           rv.next(kNV);
         }
       }
-      umma_commit(fin);
+      if (elect_one()) umma_commit(fin);
+      __syncwarp();
       mbar_wait(fin, 0u, kErrAttnDrain, kWaitLimitNs / 10);  // nothing of the tensor cores is under way past here
     }
     __syncwarp();

@@ -9,10 +9,12 @@
 // dim 128 and its 16384 exponentials as many cycles of the exponential unit; K and V come in once for both.
 //
 // Two row tiles alternate ("pair"): while one's softmax runs, the tensor cores do the other's products. Each has its
-// own warpgroup, S buffer and O. One row tile ("lone"): the S buffers take turns over the token tiles and each
-// warpgroup takes 64 of a tile's 128 tokens of every row; the two threads of a row share its reference (moved
-// together, through shared memory) and O, and add their sums at the end. Either way product v of the sequence uses S
-// buffer v % 2, and S of v + 2 is issued right after PV of v, whose P stands in that buffer.
+// own warpgroup and O. One row tile ("lone"): each warpgroup takes 64 of a tile's 128 tokens of every row; the two
+// threads of a row share its reference (moved together, through shared memory) and O, and add their sums at the end.
+// Either way there is one S, which is free again as soon as its scores are in registers, and two places for P (product
+// v of the sequence uses place v % 2): S of v + 1 is issued once S of v has been read, before PV of v - 1, so the next
+// scores are under way through the whole of a softmax. (With P over S in two buffers, S of v + 2 had to wait for PV of
+// v: 1.1 us of each 2.5 us were spent waiting for it.)
 //
 // References, partials, runs and entries that must not be seen are as in tree_attn.cuh.
 #pragma once
@@ -31,10 +33,10 @@ struct WideShape {
   static constexpr int kStage = kTok * kDim * 2;
   static constexpr int kQ = 128 * kDim * 2;  // one row tile
   static constexpr int kNK = kDim == 64 ? 4 : 2, kNV = kNK;
-  static constexpr int kTmem = 512;          // S [2][128], O [2][kDim]
+  static constexpr int kTmem = 512;          // S [128], P [2][64], O [2][kDim]
   static constexpr int kOffV = kNK * kStage, kOffQ = kOffV + kNV * kStage, kOffSmall = kOffQ + 2 * kQ;
   // mask words [256][9] (the ninth zero), exchange [2][128], scan sums, barriers
-  static constexpr int kSmall = 256 * 9 * 4 + 2 * 128 * 4 + 64 + (2 * kNK + 2 * kNV + 10) * 8 + 64;
+  static constexpr int kSmall = 256 * 9 * 4 + 2 * 128 * 4 + 64 + (2 * kNK + 2 * kNV + 11) * 8 + 64;
   static constexpr int kSmem = 1024 + kOffSmall + kSmall;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -56,6 +58,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
       : "=f"(r.x), "=f"(r.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
+}
+
+// 32 bytes, 32-byte aligned.
+__device__ __forceinline__ void st_global_v8(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]),
+               "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
 }
 
 // 16 bytes from global to shared memory without a register; zeros where `live` is false.
@@ -107,19 +116,21 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
   uint64_t* s_full = v_empty + kNV;  // [2]
   uint64_t* p_full = s_full + 2;     // [2], 256 arrivals: one a thread (lone) or two (pair)
   uint64_t* pv_done = p_full + 2;    // [2]
-  uint64_t* q_full = pv_done + 2;
+  uint64_t* s_read = pv_done + 2;    // 256 arrivals as p_full's
+  uint64_t* q_full = s_read + 1;
   uint64_t* fin = q_full + 1;
   int* start = reinterpret_cast<int*>(fin + 1);  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start + 2);
   int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     prefetch_tensormap(&tmk);
     prefetch_tensormap(&tmv);
     for (int i = 0; i < kNK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
     for (int i = 0; i < kNV; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 256), mbar_init(&pv_done[i], 1);
+    mbar_init(s_read, 256);
     mbar_init(q_full, 256);
     mbar_init(fin, 1);
     fence_mbar_init();
@@ -128,15 +139,15 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
   pdl_launch_dependents();
   pdl_wait();
   const AttnPlan plan = attn_plan<Sh::kThreads, kTok, Sh::kRows>(a, sums, start);
-  const uint32_t tmem = *tmem_slot;
-  const uint32_t tmem_o = tmem + 256;
+  const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(*tmem_slot)));
+  const uint32_t tmem_p = tmem + 128, tmem_o = tmem + 256;
 
   if (warp == 0) {
     if (plan.work)
       attn_produce<kTok, Sh::kRows, kDim, kNK, kNV>(a, plan, &tmk, &tmv, ring_k, ring_v, k_full, k_empty, v_full, v_empty);
   } else if (warp == 1) {
     // ---- UMMA issue --------------------------------------------------------------------------------
-    if (plan.work && lane == 0) {
+    if (uniform(plan.work)) {
       Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
       AttnSeg s;
       constexpr uint32_t kType = (1u << 4) | (8u << 24) | (kHalf ? 0u : ((1u << 7) | (1u << 10)));
@@ -147,55 +158,62 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
       Ring rk, rv;
       uint32_t seg_phase = 0, v0 = 0;  // products before this segment
       bool ok = true;
-      while (ok && walk.next(a, s)) {
-        ok = mbar_wait(q_full, seg_phase, kErrAttnMma);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrAttnMma)) != 0; };
+      while (ok && uniform(walk.next(a, s))) {
+        const int pair = uniform(s.r.rows - s.row0 > 128 ? 1 : 0);
+        const int products = uniform((s.i1 - s.i0) << pair);
+        ok = wait(q_full, seg_phase);
         seg_phase ^= 1u;
         if (!ok) break;
         tc_fence_after();
-        const int pair = s.r.rows - s.row0 > 128 ? 1 : 0;
-        const int products = (s.i1 - s.i0) << pair;
         // The first (or only) row tile's product waits for a K tile, the last releases it; V alike.
         auto issue_s = [&](int v) {
           const int tile = pair & v;
-          if (tile == 0 && !mbar_wait(&k_full[rk.slot], rk.phase, kErrAttnMma)) return false;
+          if (tile == 0 && !wait(&k_full[rk.slot], rk.phase)) return false;
           tc_fence_after();
-          const uint64_t dk = k_bits | ((smem_u32(ring_k + rk.slot * Sh::kStage) & 0x3FFFFu) >> 4);
-          const uint64_t dq = umma_desc_sw128(smem_u32(q_s + tile * Sh::kQ));
-          const uint32_t buffer = (v0 + v) & 1u;
+          if (elect_one()) {
+            const uint64_t dk = k_bits | ((smem_u32(ring_k + rk.slot * Sh::kStage) & 0x3FFFFu) >> 4);
+            const uint64_t dq = umma_desc_sw128(smem_u32(q_s + tile * Sh::kQ));
 #pragma unroll
-          for (int h = 0; h < kHalves; ++h)
+            for (int h = 0; h < kHalves; ++h)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              umma_bf16(tmem + buffer * 128, dq + ((h * 128 * 128) >> 4) + 2 * k, dk + ((h * 1024) >> 4) + 2 * k, idesc_s, (h | k) != 0);
-          if (tile == pair) {
-            umma_commit(&k_empty[rk.slot]);
-            rk.next(kNK);
+              for (int k = 0; k < 4; ++k)
+                umma_bf16(tmem, dq + ((h * 128 * 128) >> 4) + 2 * k, dk + ((h * 1024) >> 4) + 2 * k, idesc_s, (h | k) != 0);
+            if (tile == pair) umma_commit(&k_empty[rk.slot]);
+            umma_commit(&s_full[(v0 + v) & 1u]);
           }
-          umma_commit(&s_full[buffer]);
+          __syncwarp();
+          if (tile == pair) rk.next(kNK);
           return true;
         };
-        ok = issue_s(0) && (products < 2 || issue_s(1));
-        for (int v = 0; ok && v < products; ++v) {
-          const int tile = pair & v;
+        ok = issue_s(0);
+        for (int u = 0; ok && u <= products; ++u) {
+          if (u + 1 < products) {
+            ok = wait(s_read, (v0 + u) & 1u) && issue_s(u + 1);
+            if (!ok) break;
+          }
+          if (u == 0) continue;
+          const int v = u - 1, tile = pair & v;
           const uint32_t n = v0 + v, buffer = n & 1u;
-          ok = mbar_wait(&p_full[buffer], (n >> 1) & 1u, kErrAttnMma) && (tile != 0 || mbar_wait(&v_full[rv.slot], rv.phase, kErrAttnMma));
+          ok = wait(&p_full[buffer], (n >> 1) & 1u) && (tile != 0 || wait(&v_full[rv.slot], rv.phase));
           if (!ok) break;
           tc_fence_after();
-          const uint64_t dv = v_bits | ((smem_u32(ring_v + rv.slot * Sh::kStage) & 0x3FFFFu) >> 4);
+          if (elect_one()) {
+            const uint64_t dv = v_bits | ((smem_u32(ring_v + rv.slot * Sh::kStage) & 0x3FFFFu) >> 4);
 #pragma unroll
-          for (int k = 0; k < kTok / 16; ++k)
-            umma_ts(tmem_o + tile * kDim, tmem + buffer * 128 + k * 8, dv + ((k * 16 * kDim * 2) >> 4), idesc_o,
-                    (v > pair || k > 0) ? 1u : 0u);
-          if (tile == pair) {
-            umma_commit(&v_empty[rv.slot]);
-            rv.next(kNV);
+            for (int k = 0; k < kTok / 16; ++k)
+              umma_ts(tmem_o + tile * kDim, tmem_p + buffer * 64 + k * 8, dv + ((k * 16 * kDim * 2) >> 4), idesc_o,
+                      (v > pair || k > 0) ? 1u : 0u);
+            if (tile == pair) umma_commit(&v_empty[rv.slot]);
+            umma_commit(&pv_done[buffer]);
           }
-          umma_commit(&pv_done[buffer]);
-          if (v + 2 < products) ok = issue_s(v + 2);
+          __syncwarp();
+          if (tile == pair) rv.next(kNV);
         }
         v0 += products;
       }
-      umma_commit(fin);
+      if (elect_one()) umma_commit(fin);
+      __syncwarp();
       mbar_wait(fin, 0u, kErrAttnDrain, kWaitLimitNs / 10);  // nothing of the tensor cores is under way past here
     }
     __syncwarp();
@@ -210,26 +228,32 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
     AttnCross cross = {};
     if (plan.work) {
       Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
-      AttnSeg s;
+      AttnSeg s, next;
       uint32_t v0 = 0, v_slot = 0, v_phase = 0;
       bool ok = true;
-      while (ok && walk.next(a, s)) {
+      // Q of a segment: a thread a 16-byte chunk at a time, all of them on their way at once.
+      constexpr int kChunks = kDim / 8;
+      auto q_at = [&](int r, int ch) {
+        return smem_u32(q_s) + (r >> 7) * Sh::kQ + (ch >> 3) * (128 * 128) + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4);
+      };
+      auto q_rows = [&](const AttnSeg& s) { return s.r.rows - s.row0 > 128 ? 256 : 128; };
+      auto load_q = [&](const AttnSeg& s) {
+        const int last = min(Sh::kRows, s.r.rows - s.row0) - 1;
+        for (int i = tid; i < q_rows(s) * kChunks; i += 256) {
+          const int r = i / kChunks, ch = i % kChunks, row = s.row0 + min(r, last), t = attn_token(a, row);
+          cp_async16(q_at(r, ch), a.q + (s.r.first + t) * a.q_token + (s.head * g + row - t * g) * a.q_head + ch * 8, r <= last);
+        }
+      };
+      bool more = walk.next(a, next);
+      if (more) load_q(next);
+      while (ok && more) {
+        s = next;
         const int rows = min(Sh::kRows, s.r.rows - s.row0);
         const bool pair = rows > 128;
         const int row = pair ? wg * 128 + tl : tl;                   // this thread's row of the unit
         const bool mine = row < rows;
-        const int t = mine ? attn_token(a, s.row0 + row) : 0;
-        bar_named(8, 256);  // every thread is done with the last segment's arrays
-        // Q: a thread a 16-byte chunk at a time, all of them on their way at once.
-        const int q_rows = pair ? 256 : 128;
-        constexpr int kChunks = kDim / 8;
-        auto q_at = [&](int r, int ch) {
-          return smem_u32(q_s) + (r >> 7) * Sh::kQ + (ch >> 3) * (128 * 128) + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4);
-        };
-        for (int i = tid; i < q_rows * kChunks; i += 256) {
-          const int r = i / kChunks, ch = i % kChunks, rr = min(r, rows - 1), tr = attn_token(a, s.row0 + rr);
-          cp_async16(q_at(r, ch), a.q + (s.r.first + tr) * a.q_token + (s.head * g + s.row0 + rr - tr * g) * a.q_head + ch * 8, r < rows);
-        }
+        const int t = mine ? attn_token(a, s.row0 + row) : 0, h = s.head * g + s.row0 + row - t * g;
+        bar_named(8, 256);  // every thread is done with the last segment's words
         if (wg == 0 || pair) {
           const int nw = (s.r.drafted + 31) >> 5;
           for (int w = 0; w < nw; ++w) words[row * 9 + w] = mine ? attn_seen_word(a, s.r, t, w) : 0u;
@@ -238,7 +262,7 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
         if (tid == 0) *odd_v = 0;
         cp_async_wait();
         if (a.q_flip) {  // a negative scale: this thread's own chunks with the other sign
-          for (int i = tid; i < q_rows * kChunks; i += 256) {
+          for (int i = tid; i < q_rows(s) * kChunks; i += 256) {
             const uint32_t at = q_at(i / kChunks, i % kChunks);
             const uint4 v = ld_shared_v4u(at);
             st_shared_v4u(at, v.x ^ a.q_flip, v.y ^ a.q_flip, v.z ^ a.q_flip, v.w ^ a.q_flip);
@@ -259,12 +283,23 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           constexpr bool kPair = kN == 128;
           const uint32_t n = v0 + v, buffer = n & 1u;
           const int i = s.i0 + (kPair ? v >> 1 : v), col0 = kPair ? 0 : wg * 64;
+          const bool edge = (i + 1) * kTok > s.r.ctx;  // the tile reaches past the context
+          if (wg == 0 && edge) {
+            const bool ragged = (i + 1) * kTok > s.r.kv, drafted = s.r.drafted > 1;
+            if (ragged || drafted) {
+              ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
+              const int pos = i * kTok + tl;
+              attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), tl, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);
+              fence_proxy_async_shared();
+            }
+          }
           ok = mbar_wait(&s_full[buffer], (n >> 1) & 1u, kErrAttnSoftmax) && ok;
           tc_fence_after();
-          const uint32_t ts = tmem + buffer * 128 + lanes;
           float x[kN];
-          wide_ld<kN>(ts + col0, x);
-          const bool edge = (i + 1) * kTok > s.r.ctx;  // the tile reaches past the context
+          wide_ld<kN>(tmem + col0 + lanes, x);
+          tc_fence_before();
+          if (kPair) mbar_arrive_n(s_read, 2);
+          else mbar_arrive(s_read);
           if (edge) {
 #pragma unroll
             for (int cc = 0; cc < kN; cc += 32) {
@@ -277,8 +312,7 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
 #pragma unroll
           for (int k = 4; k < kN; ++k) m[k & 3] = fmaxf(m[k & 3], x[k]);
           float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c;
-          // Whether this warp (pair) or any softmax thread (lone; S has been read by both warpgroups after this) has a
-          // reference to move.
+          // Whether this warp (pair) or any softmax thread (lone) has a reference to move.
           const bool past = top - ref > kAttnSlack || !ok;
           if (kPair ? __any_sync(0xffffffffu, past) : bar_any(8, 256, past)) {
             if (kPair ? __any_sync(0xffffffffu, !ok) : bar_any(8, 256, !ok)) return false;
@@ -292,11 +326,9 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
             ref = now;
             l *= f;
             if (v >= step) {
-              // O is whole up to the product before: the pair's last of this row tile came before S, the lone one's not.
-              if (!kPair) {
-                ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax) && ok;
-                tc_fence_after();
-              }
+              // O has to be whole up to this row tile's product before.
+              ok = mbar_wait(&pv_done[(n - step) & 1u], ((n - step) >> 1) & 1u, kErrAttnSoftmax) && ok;
+              tc_fence_after();
               const int d0 = kPair ? 0 : wg * (kDim / 2), d1 = kPair ? kDim : d0 + kDim / 2;
 #pragma unroll 1
               for (int d = d0; d < d1; d += 16) {
@@ -309,7 +341,9 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
               attn_st_wait();
             }
           }
-          // P, rounded, over S's columns: 32 scores become 16 words.
+          // P, rounded, once its place is free: 32 scores become 16 words.
+          if (v >= 2) ok = mbar_wait(&pv_done[buffer], ((n - 2) >> 1) & 1u, kErrAttnSoftmax) && ok;
+          tc_fence_after();
           float2 sum = {0.f, 0.f};
           const float2 cc2 = {c, c}, mm2 = {-ref, -ref};
 #pragma unroll
@@ -322,19 +356,10 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
               add16x2<kHalf>(w, sum.x, sum.y);
               p[k] = __uint_as_float(w);
             }
-            attn_st16(ts + ((col0 + cc) >> 1), p);
+            attn_st16(tmem_p + buffer * 64 + ((col0 + cc) >> 1) + lanes, p);
           }
           l += sum.x + sum.y;
           attn_st_wait();
-          if (wg == 0) {
-            const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && s.r.drafted > 1;
-            if (ragged || drafted) {
-              ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
-              const int pos = i * kTok + tl;
-              attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), tl, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);
-              fence_proxy_async_shared();
-            }
-          }
           if (++v_slot == kNV) v_slot = 0, v_phase ^= 1u;
           tc_fence_before();
           if (kPair) mbar_arrive_n(&p_full[buffer], 2);
@@ -360,6 +385,8 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         v0 += products;
+        more = walk.next(a, next);
+        if (more) load_q(next);  // this segment's products, the readers of Q, are done
         if (!pair) l += swap[(wg ^ 1) * 128 + tl];
         const bool whole = s.i0 == 0 && s.i1 == s.r.tiles;
         const long long slot = (static_cast<long long>(blockIdx.x) * 2 + (s.i0 > 0 ? 0 : 1)) * Sh::kRows + row;
@@ -368,63 +395,54 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           cross.first = s.r.first, cross.row0 = s.row0, cross.rows = rows, cross.head = s.head;
           cross.last = plan.runs.of(s.unit0 + s.r.tiles - 1);
         }
-        const float inv = !whole ? 1.f : (l == 0.f ? 0.f : 1.f / l);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
         const int odd = *odd_v;
-        // Rows leave through Q's place (its products are done), half of dim at a time: [128 rows][kDim / 2] FP32 a
-        // warpgroup, 16-byte chunks swizzled by the row, so that a warp writes whole lines.
-        constexpr int kPart = kDim / 2, kPieces = kPart / 4;
-        const uint32_t stage = smem_u32(q_s) + wg * Sh::kQ;
-        for (int d = pair ? 0 : wg * kPart; d < (pair ? kDim : (wg + 1) * kPart); d += kPart) {
-          bar_named(1 + wg, 128);
+        // A thread writes its own row.
+        const int d0 = pair ? 0 : wg * (kDim / 2), d1 = pair ? kDim : d0 + kDim / 2;
+        uint16_t* out = a.out + (s.r.first + t) * a.out_token + h * a.out_head;
+        const uint16_t* gate = a.gate ? a.gate + (s.r.first + t) * a.gate_token + h * a.gate_head : nullptr;
+        float* part = a.part_o + slot * kDim;
 #pragma unroll 1
-          for (int e = 0; e < kPart; e += 16) {
-            float o[16];
-            wide_ld<16>(o_base + d + e, o);
-            if (odd && mine) {
-              // Put the non-finite entries back for the rows that see them.
-              const int j0 = max(s.i0 * kTok - s.r.ctx, 0), j1 = min(min(s.i1 * kTok, s.r.kv) - s.r.ctx, s.r.drafted);
-              for (int j = j0; j < j1; ++j) {
-                if (!((words[row * 9 + (j >> 5)] >> (j & 31)) & 1u)) continue;
-                const int p = s.r.ctx + j;
-                const long long page = a.table[s.b * a.table_row + p / a.page];
-                if (page < 0 || page >= a.pages) continue;
-                const uint16_t* src = a.v_pages + page * a.v_page + s.head * a.v_head + (p % a.page) * a.v_slot + d + e;
+        for (int d = d0; d < d1; d += 16) {
+          uint4 g0 = make_uint4(0u, 0u, 0u, 0u), g1 = g0;
+          if (whole && gate && mine) g0 = __ldg(reinterpret_cast<const uint4*>(gate + d)), g1 = __ldg(reinterpret_cast<const uint4*>(gate + d) + 1);
+          float o[16];
+          wide_ld<16>(o_base + d, o);
+          if (!mine) continue;
+          if (odd) {
+            // Put the non-finite entries back for the rows that see them.
+            const int j0 = max(s.i0 * kTok - s.r.ctx, 0), j1 = min(min(s.i1 * kTok, s.r.kv) - s.r.ctx, s.r.drafted);
+            for (int j = j0; j < j1; ++j) {
+              if (!((words[row * 9 + (j >> 5)] >> (j & 31)) & 1u)) continue;
+              const int p = s.r.ctx + j;
+              const long long page = a.table[s.b * a.table_row + p / a.page];
+              if (page < 0 || page >= a.pages) continue;
+              const uint16_t* src = a.v_pages + page * a.v_page + s.head * a.v_head + (p % a.page) * a.v_slot + d;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                  const float x = lo16<kHalf>(src[k]);
-                  if (!(fabsf(x) < __int_as_float(0x7f800000))) o[k] += x;
-                }
+              for (int k = 0; k < 16; ++k) {
+                const float x = lo16<kHalf>(src[k]);
+                if (!(fabsf(x) < __int_as_float(0x7f800000))) o[k] += x;
               }
-            }
-#pragma unroll
-            for (int k = 0; k < 16; k += 4) {
-              const int ch = (e + k) >> 2;
-              st_shared_v4u(stage + tl * (kPart * 4) + ((ch ^ (tl & (kPieces - 1))) << 4), __float_as_uint(o[k] * inv),
-                            __float_as_uint(o[k + 1] * inv), __float_as_uint(o[k + 2] * inv), __float_as_uint(o[k + 3] * inv));
             }
           }
-          bar_named(1 + wg, 128);
-          const int first = pair ? wg * 128 : 0;  // the unit's row of this warpgroup's row 0
-          for (int u = tid & 127; u < 128 * kPieces; u += 128) {
-            const int r = u / kPieces, ch = u % kPieces, of = first + r;
-            if (of >= rows) break;  // rows ascend with u
-            const float4 o = ld_shared_v4(stage + r * (kPart * 4) + ((ch ^ (r & (kPieces - 1))) << 4));
-            if (whole) {
-              const int tr = attn_token(a, s.row0 + of), hr = s.head * g + s.row0 + of - tr * g;
-              float e[4] = {o.x, o.y, o.z, o.w};
-              if (a.gate) {
-                const uint2 gw = __ldg(reinterpret_cast<const uint2*>(a.gate + (s.r.first + tr) * a.gate_token + hr * a.gate_head + d + ch * 4));
-                e[0] = __fdividef(e[0], 1.f + __expf(-lo16<kHalf>(gw.x)));
-                e[1] = __fdividef(e[1], 1.f + __expf(-hi16<kHalf>(gw.x)));
-                e[2] = __fdividef(e[2], 1.f + __expf(-lo16<kHalf>(gw.y)));
-                e[3] = __fdividef(e[3], 1.f + __expf(-hi16<kHalf>(gw.y)));
+          if (whole) {
+            const uint32_t gw[8] = {g0.x, g0.y, g0.z, g0.w, g1.x, g1.y, g1.z, g1.w};
+            uint32_t w[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              float e0 = o[2 * k] * inv, e1 = o[2 * k + 1] * inv;
+              if (gate) {
+                e0 = __fdividef(e0, 1.f + __expf(-lo16<kHalf>(gw[k])));
+                e1 = __fdividef(e1, 1.f + __expf(-hi16<kHalf>(gw[k])));
               }
-              *reinterpret_cast<uint2*>(a.out + (s.r.first + tr) * a.out_token + hr * a.out_head + d + ch * 4) =
-                  make_uint2(pack16x2<kHalf>(e[0], e[1]), pack16x2<kHalf>(e[2], e[3]));
-            } else {
-              const long long at = (static_cast<long long>(blockIdx.x) * 2 + (s.i0 > 0 ? 0 : 1)) * Sh::kRows + of;
-              *reinterpret_cast<float4*>(a.part_o + at * kDim + d + ch * 4) = o;
+              w[k] = pack16x2<kHalf>(e0, e1);
             }
+            // out is 16-byte aligned, not 32: two stores.
+            reinterpret_cast<uint4*>(out + d)[0] = make_uint4(w[0], w[1], w[2], w[3]);
+            reinterpret_cast<uint4*>(out + d)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+          } else {
+            st_global_v8(part + d, o);
+            st_global_v8(part + d + 8, o + 8);
           }
         }
         tc_fence_before();
