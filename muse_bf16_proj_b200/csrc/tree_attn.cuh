@@ -43,9 +43,11 @@
 namespace muse {
 
 constexpr unsigned int kErrAttnDraft = 0xB01, kErrAttnTable = 0xB02, kErrAttnPage = 0xB03;
-constexpr unsigned int kErrAttnProducer = 0xB11, kErrAttnMma = 0xB12, kErrAttnSoftmax = 0xB13, kErrAttnDrain = 0xB14;
+constexpr unsigned int kErrAttnProducer = 0xB11, kErrAttnMma = 0xB12, kErrAttnSoftmax = 0xB13, kErrAttnDrain = 0xB14,
+                       kErrAttnLoader = 0xB15;
 
 constexpr float kAttnSlack = 8.f;   // log2 of how far a score may pass its row's reference maximum
+constexpr int kAttnEnds = 2;        // what a row tile's beginning and end cost, in token tiles, when runs are cut
 constexpr float kAttnUnseen = -1e30f;  // reference of a row that has seen nothing: below every score, and finite
 
 struct AttnArgs {
@@ -88,7 +90,7 @@ struct AttnShape {
   static constexpr int kTok = 128 * kTG;                          // cached tokens a tile
   static constexpr int kCols = kRows / kCG;
   static constexpr int kSoft = 128 * kTG * kCG;                   // softmax threads
-  static constexpr int kThreads = 64 + kSoft;
+  static constexpr int kThreads = 64 + kSoft + 32;                // producer, UMMA, softmax, row loader
   static constexpr int kStage = kTok * kDim * 2;                  // one K or V tile
   static constexpr int kQ = kRows * kDim * 2;
   static constexpr int kP = kTok * kRows * 2;
@@ -98,8 +100,8 @@ struct AttnShape {
   static constexpr int kTmemO = 2 * kTG * kRows;                  // after two buffers of S^T
   static constexpr int kTmem = kTmemO + kRows <= 64 ? 64 : (kTmemO + kRows <= 128 ? 128 : (kTmemO + kRows <= 256 ? 256 : 512));
   static constexpr int kOffV = kNK * kStage, kOffQ = kOffV + kNV * kStage, kOffP = kOffQ + kQ, kOffSmall = kOffP + kNP * kP;
-  // ref, rescale, 1 / sum and row ids [kRows]; red [4 kTG][kRows]; mask words [kRows][8]; barriers.
-  static constexpr int kSmall = kRows * 4 * 4 + 4 * kTG * kRows * 4 + kRows * 32 + (2 * kNK + 2 * kNV + 9) * 8 + 64;
+  // ref, rescale, 1 / sum [kRows]; row ids [2][kRows]; red [4 kTG][kRows]; mask words [2][kRows][9]; segments; barriers.
+  static constexpr int kSmall = kRows * 4 * 5 + 4 * kTG * kRows * 4 + kRows * 72 + 128 + (2 * kNK + 2 * kNV + 11) * 8 + 64;
   static constexpr int kSmem = 1024 + kOffSmall + kSmall;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -107,6 +109,7 @@ struct AttnShape {
 struct AttnReq {
   int first, drafted, ctx, kv, tiles, rows;  // first token, drafted tokens, context, entries, token tiles, rows a kv head
   int units;                                 // kv heads x row tiles
+  int cost;                                  // of a unit, in token tiles (0: nothing to do)
 };
 
 // A request's sizes, clamped to what may be touched whatever the device arrays hold.
@@ -124,65 +127,70 @@ __device__ __forceinline__ AttnReq attn_request(const AttnArgs& a, int b, bool r
   if (report && t > 0 && want > have) report_error(kErrAttnTable);
   r.kv = static_cast<int>(min(want, have));
   r.tiles = t > 0 ? (r.kv + kTok - 1) / kTok : 0;
+  r.cost = r.tiles > 0 ? r.tiles + kAttnEnds : 0;
   r.rows = t * (a.heads / a.kv_heads);
   r.units = a.kv_heads * ((r.rows + kRows - 1) / kRows);
   return r;
 }
 
-// `total` tiles over at most `ctas` runs of at least one tile, the first `more` one tile longer.
+// `total` of cost over at most `ctas` runs, the first `more` one longer.
 struct AttnRuns {
   int runs, per, more;
   __device__ __forceinline__ AttnRuns(int total, int ctas) : runs(min(total, ctas)), per(0), more(0) {
     if (runs > 0) per = total / runs, more = total - per * runs;
   }
   __device__ __forceinline__ int start(int c) const { return c * per + min(c, more); }
-  // The run that holds tile w.
+  // The run that holds position w.
   __device__ __forceinline__ int of(int w) const {
     const int longer = more * (per + 1);
     return w < longer ? w / (per + 1) : more + (w - longer) / per;
   }
 };
 
-// Walks a CTA's run segment by segment (a segment: consecutive token tiles of one row tile and kv head).
+// Walks a CTA's run segment by segment (a segment: consecutive token tiles of one row tile and kv head). A unit's
+// positions are kAttnEnds of its ends, then its tiles.
 struct AttnSeg {
   int b, head, row0, i0, i1;  // request, kv head, first row, token tiles [i0, i1)
-  int unit0;                  // tiles before this unit, over all requests
+  int unit0;                  // position of the unit's first tile
   AttnReq r;
 };
 template <int kTok, int kRows>
 struct AttnWalk {
-  int left, base;  // tiles left in the run; tiles before request b
-  int unit, b, i;
+  int left, base;  // of the run; positions before request b
+  int unit, b, at;  // unit of the request, position in it
   AttnReq r;
   __device__ __forceinline__ AttnWalk(const AttnArgs& a, int b0, int base0, int w0, int w1)
-      : left(w1 - w0), base(base0), unit(0), b(b0), i(0) {
+      : left(w1 - w0), base(base0), unit(0), b(b0), at(0) {
     r = attn_request<kTok, kRows>(a, b, false);
     const int off = w0 - base;
-    unit = off / r.tiles;
-    i = off - unit * r.tiles;
+    unit = off / r.cost;
+    at = off - unit * r.cost;
   }
   __device__ __forceinline__ bool next(const AttnArgs& a, AttnSeg& s) {
-    if (left <= 0) return false;
-    while (unit >= r.units || r.tiles == 0) {
-      base += r.units * r.tiles;
-      if (++b >= a.requests) return false;
-      r = attn_request<kTok, kRows>(a, b, false);
-      unit = 0;
-      i = 0;
+    while (left > 0) {
+      while (unit >= r.units || r.cost == 0) {
+        base += r.units * r.cost;
+        if (++b >= a.requests) return false;
+        r = attn_request<kTok, kRows>(a, b, false);
+        unit = 0;
+        at = 0;
+      }
+      const int take = min(left, r.cost - at);
+      s.i0 = max(at - kAttnEnds, 0);
+      s.i1 = max(at + take - kAttnEnds, 0);
+      s.b = b;
+      s.r = r;
+      // Row tiles of one kv head follow one another, so that CTAs that share cached tokens run side by side.
+      const int row_tiles = (r.rows + kRows - 1) / kRows;
+      s.head = row_tiles == 1 ? unit : unit / row_tiles;
+      s.row0 = (unit - s.head * row_tiles) * kRows;
+      s.unit0 = base + unit * r.cost + kAttnEnds;
+      left -= take;
+      ++unit;
+      at = 0;
+      if (s.i1 > s.i0) return true;
     }
-    s.b = b;
-    s.r = r;
-    // Row tiles of one kv head follow one another, so that CTAs that share cached tokens run side by side.
-    const int row_tiles = (r.rows + kRows - 1) / kRows;
-    s.head = row_tiles == 1 ? unit : unit / row_tiles;
-    s.row0 = (unit - s.head * row_tiles) * kRows;
-    s.unit0 = base + unit * r.tiles;
-    s.i0 = i;
-    s.i1 = min(r.tiles, i + left);
-    left -= s.i1 - s.i0;
-    ++unit;
-    i = 0;
-    return true;
+    return false;
   }
 };
 
@@ -294,7 +302,7 @@ __device__ __forceinline__ uint32_t attn_row(int token, int halves) { return sta
 // Where a CTA's run starts: every CTA scans the requests (a run of requests a thread), none waits for another.
 struct AttnPlan {
   AttnRuns runs;
-  int w0, w1, b0, s0;  // the run [w0, w1); its first request and the tiles before that
+  int w0, w1, b0, s0;  // the run [w0, w1); its first request and the positions before that
   bool work;
 };
 template <int kThreads, int kTok, int kRows>
@@ -305,7 +313,7 @@ __device__ __forceinline__ AttnPlan attn_plan(const AttnArgs& a, int* sums, int*
   const int b_lo = min(static_cast<int>(threadIdx.x) * each, a.requests), b_hi = min(b_lo + each, a.requests);
   for (int b = b_lo; b < b_hi; ++b) {
     const AttnReq r = attn_request<kTok, kRows>(a, b, blockIdx.x == 0);
-    mine += r.units * r.tiles;
+    mine += r.units * r.cost;
   }
   int upto = mine;
 #pragma unroll
@@ -329,8 +337,8 @@ __device__ __forceinline__ AttnPlan attn_plan(const AttnArgs& a, int* sums, int*
     if (each > 1) {
       for (;; ++b) {
         const AttnReq r = attn_request<kTok, kRows>(a, b, false);
-        if (p.w0 < at + r.units * r.tiles) break;
-        at += r.units * r.tiles;
+        if (p.w0 < at + r.units * r.cost) break;
+        at += r.units * r.cost;
       }
     }
     start[0] = b, start[1] = at;
@@ -449,11 +457,68 @@ __device__ __forceinline__ uint32_t attn_seen_word(const AttnArgs& a, const Attn
   return v & (n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u));
 }
 
+// 16 bytes from global to shared memory without a register; zeros where `live` is false.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// The row loader (kLanes threads of their own): for each segment of the run its description, mask words and row ids
+// (two places in turn) and Q, as soon as the last product that reads the segment before's Q is done: while that segment's
+// softmax, second products and end still run (a segment's first scores wait for it no longer than that). q_full tells the others (kLanes arrivals); a segment without tiles ends
+// the run. Q is [row tiles of kTile rows][halves][kTile][64 dims] swizzled; `fill` rows of it are written, zeros past the rows.
+template <int kTok, int kRows, int kTile, int kDim, int kLanes>
+__device__ __forceinline__ void attn_load_rows(const AttnArgs& a, const AttnPlan& plan, int me, uint8_t* q_s, AttnSeg* segs, uint32_t* words,
+                                               int* row_id, uint64_t* q_full, uint64_t* q_empty, uint64_t* seg_done) {
+  constexpr int kChunks = kDim / 8;
+  const int g = a.heads / a.kv_heads;
+  AttnWalk<kTok, kRows> walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
+  AttnSeg s;
+  for (int k = 0;; ++k) {
+    const bool more = walk.next(a, s);
+    if (!more) s.i0 = s.i1 = 0;
+    // This place's last user, two segments ago, is done with it.
+    if (k > 1 && !mbar_wait(seg_done, k & 1, kErrAttnLoader)) break;
+    if (me == 0) segs[k & 1] = s;
+    if (more) {
+      const int rows = min(kRows, s.r.rows - s.row0), fill = kTile == kRows ? min(kRows, (rows + 15) & ~15) : (rows > kTile ? kRows : kTile);
+      uint32_t* w = words + (k & 1) * kRows * 9;
+      int* id = row_id + (k & 1) * kRows;
+      const int nw = (s.r.drafted + 31) >> 5;
+      for (int r = me; r < fill; r += kLanes) {
+        const int row = s.row0 + min(r, rows - 1), t = attn_token(a, row);
+        id[r] = (t << 16) | (s.head * g + row - t * g);
+        for (int j = 0; j < 9; ++j) w[r * 9 + j] = j < nw && r < rows ? attn_seen_word(a, s.r, t, j) : 0u;
+      }
+      if (k > 0 && !mbar_wait(q_empty, (k - 1) & 1, kErrAttnLoader)) break;
+      auto at = [&](int r, int ch) {
+        return smem_u32(q_s) + (r / kTile) * (kTile * kDim * 2) + (ch >> 3) * (kTile * 128) + (r & (kTile - 1)) * 128 +
+               (((ch & 7) ^ (r & 7)) << 4);
+      };
+#pragma unroll 4
+      for (int i = me; i < fill * kChunks; i += kLanes) {
+        const int r = i / kChunks, ch = i % kChunks, row = s.row0 + min(r, rows - 1), t = attn_token(a, row);
+        cp_async16(at(r, ch), a.q + (s.r.first + t) * a.q_token + (s.head * g + row - t * g) * a.q_head + ch * 8, r < rows);
+      }
+      cp_async_wait();
+      if (a.q_flip) {  // a negative scale: this thread's own chunks with the other sign
+        for (int i = me; i < fill * kChunks; i += kLanes) {
+          const uint32_t to = at(i / kChunks, i % kChunks);
+          const uint4 v = ld_shared_v4u(to);
+          st_shared_v4u(to, v.x ^ a.q_flip, v.y ^ a.q_flip, v.z ^ a.q_flip, v.w ^ a.q_flip);
+        }
+      }
+      fence_proxy_async_shared();
+    }
+    mbar_arrive(q_full);
+    if (!more) break;
+  }
+}
+
 template <bool kHalf, int kDim, int kRows>
 __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttnArgs a) {
   using Sh = AttnShape<kDim, kRows>;
-  using Walk = AttnWalk<Sh::kTok, kRows>;
   constexpr int kHalves = Sh::kHalves, kNK = Sh::kNK, kNV = Sh::kNV, kNP = Sh::kNP, kCols = Sh::kCols, kTok = Sh::kTok;
   constexpr int kTG = Sh::kTG, kSoft = Sh::kSoft;
   extern __shared__ uint8_t smem_raw[];
@@ -465,10 +530,11 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   float* ref = reinterpret_cast<float*>(smem + Sh::kOffSmall);  // reference maximum (scaled, log2)
   float* rescale = ref + kRows;
   float* inv = rescale + kRows;
-  int* row_id = reinterpret_cast<int*>(inv + kRows);             // token of the request << 16 | query head
-  float* red = reinterpret_cast<float*>(row_id + kRows);         // [4 kTG][kRows]
-  uint32_t* words = reinterpret_cast<uint32_t*>(red + 4 * kTG * kRows);  // [kRows][8]: drafted tokens a row sees
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(words + kRows * 8);
+  int* row_ids = reinterpret_cast<int*>(inv + kRows);            // [2][kRows]: token of the request << 16 | query head
+  float* red = reinterpret_cast<float*>(row_ids + 2 * kRows);    // [4 kTG][kRows]
+  uint32_t* all_words = reinterpret_cast<uint32_t*>(red + 4 * kTG * kRows);  // [2][kRows][9]: drafted tokens a row sees
+  AttnSeg* segs = reinterpret_cast<AttnSeg*>(all_words + 2 * kRows * 9);     // [2]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(segs) + 16;
   uint64_t* k_empty = k_full + kNK;
   uint64_t* v_full = k_empty + kNK;
   uint64_t* v_empty = v_full + kNV;
@@ -478,10 +544,12 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   // would by then name the next phase.
   uint64_t* pv_done = p_full + 2;
   uint64_t* q_full = pv_done + 2;
-  uint64_t* fin = q_full + 1;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* seg_done = q_empty + 1;
+  uint64_t* fin = seg_done + 1;
   int* start_b = reinterpret_cast<int*>(fin + 1);  // [2]: the run's first request, and the tiles before it
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start_b + 2);
-  int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);  // a drafted token of this segment has a non-finite V entry
+  int* odd_vs = reinterpret_cast<int*>(tmem_slot + 1);  // [2], by segment: a drafted token has a non-finite V entry
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -490,7 +558,10 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     for (int i = 0; i < kNK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
     for (int i = 0; i < kNV; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kSoft), mbar_init(&pv_done[i], 1);
-    mbar_init(q_full, kSoft);
+    mbar_init(q_full, 32);
+    mbar_init(q_empty, 1);
+    mbar_init(seg_done, kSoft);
+    odd_vs[0] = odd_vs[1] = 0;
     mbar_init(fin, 1);
     fence_mbar_init();
   }
@@ -508,8 +579,6 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   } else if (warp == 1) {
     // ---- UMMA issue --------------------------------------------------------------------------------
     if (uniform(plan.work)) {
-      Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
-      AttnSeg s;
       constexpr uint32_t kType = kHalf ? 0u : ((1u << 7) | (1u << 10));
       constexpr uint32_t kShape = (1u << 4) | (static_cast<uint32_t>(kRows >> 3) << 17) | (8u << 24);
       constexpr uint32_t idesc_s = kShape | kType, idesc_o = kShape | kType | (1u << 15) | (1u << 16);
@@ -518,10 +587,10 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       constexpr uint64_t v_bits = attn_desc_bits(128, 1024 * kHalves, kHalves > 1 ? 1024 : 0);
       constexpr uint64_t p_bits = attn_desc_bits(kPRow, 8 * kPRow, 0);
       Ring rk, rv;
-      uint32_t seg_phase = 0, n = 0;
+      uint32_t n = 0;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrAttnMma)) != 0; };
-      auto issue_s = [&](uint32_t m) {
+      auto issue_s = [&](uint32_t m, bool last) {
         if (!wait(&k_full[rk.slot], rk.phase)) return false;
         tc_fence_after();
         if (elect_one()) {
@@ -536,21 +605,21 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
                           dq + ((h * kRows * 128) >> 4) + 2 * k, idesc_s, (h | k) != 0);
           umma_commit(&k_empty[rk.slot]);
           umma_commit(&s_full[m & 1u]);
+          if (last) umma_commit(q_empty);
         }
         __syncwarp();
         rk.next(kNK);
         return true;
       };
-      while (ok && uniform(walk.next(a, s))) {
-        const int tiles = uniform(s.i1 - s.i0);
-        ok = wait(q_full, seg_phase);
-        seg_phase ^= 1u;
-        if (!ok) break;
+      for (int k = 0;; ++k) {
+        if (!(ok = wait(q_full, k & 1))) break;
+        const int tiles = uniform(segs[k & 1].i1 - segs[k & 1].i0);
+        if (tiles == 0) break;
         tc_fence_after();
-        ok = issue_s(n);
+        ok = issue_s(n, tiles == 1);
         for (int i = 0; ok && i < tiles; ++i, ++n) {
           // The next tile's scores are under way while the softmax of this one runs.
-          if (i + 1 < tiles && !(ok = issue_s(n + 1))) break;
+          if (i + 1 < tiles && !(ok = issue_s(n + 1, i + 2 == tiles))) break;
           ok = wait(&p_full[n & 1u], (n >> 1) & 1u) && wait(&v_full[rv.slot], rv.phase);
           if (!ok) break;
           tc_fence_after();
@@ -566,12 +635,16 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           __syncwarp();
           rv.next(kNV);
         }
+        if (!ok) break;
       }
       if (elect_one()) umma_commit(fin);
       __syncwarp();
       mbar_wait(fin, 0u, kErrAttnDrain, kWaitLimitNs / 10);  // nothing of the tensor cores is under way past here
     }
     __syncwarp();
+  } else if (warp == Sh::kThreads / 32 - 1) {
+    if (plan.work)
+      attn_load_rows<kTok, kRows, kRows, kDim, 32>(a, plan, lane, q_s, segs, all_words, row_ids, q_full, q_empty, seg_done);
   } else {
     // ---- softmax: thread = one token of the tile (a TMEM lane of its token group), its group's columns ----
     const int tid = static_cast<int>(threadIdx.x) - 64;
@@ -582,57 +655,28 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     constexpr int kGroup = 128 * kTG;  // threads that share columns
     const int gtid = tid % kGroup;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const int g = a.heads / a.kv_heads;
     const float kNegInf = __int_as_float(0xff800000);
     const float c = a.scale_log2;
     AttnCross cross = {};
     if (plan.work) {
-      Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
-      AttnSeg s;
       uint32_t n = 0;  // tiles done in this run
       uint32_t v_slot = 0, v_phase = 0;
       bool ok = true;
       float l[kCols];
-      while (ok && walk.next(a, s)) {
-        // ---- the segment's rows: Q, mask words, references -----------------------------------------
+      for (int k = 0;; ++k) {
+        // ---- the segment's rows --------------------------------------------------------------------
+        ok = mbar_wait(q_full, k & 1, kErrAttnSoftmax);
+        if (bar_any(8, kSoft, !ok)) break;  // every thread is done with the last segment's arrays, too
+        const AttnSeg s = segs[k & 1];
+        if (s.i1 <= s.i0) break;
         const int rows = min(kRows, s.r.rows - s.row0);
         const int full = min(kRows, (rows + 15) & ~15);  // columns that are computed
         const int live = min(max(full - c0, 0), kCols);  // of this group
-        bar_named(8, kSoft);                             // every thread is done with the last segment's arrays
-        constexpr int kLoads = kRows * (kDim / 8) / kSoft > 0 ? kRows * (kDim / 8) / kSoft : 1;
-        uint4 qv[kLoads];
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-          const int i = tid + u * kSoft, r = i / (kDim / 8), ch = i % (kDim / 8);
-          qv[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (r < rows) {
-            const int t = attn_token(a, s.row0 + r);
-            qv[u] = __ldg(reinterpret_cast<const uint4*>(a.q + (s.r.first + t) * a.q_token +
-                                                         (s.head * g + s.row0 + r - t * g) * a.q_head + ch * 8));
-          }
-        }
-        const int nw = (s.r.drafted + 31) >> 5;
-        for (int i = tid; i < full * 8; i += kSoft) {
-          const int r = i >> 3, w = i & 7;
-          if (w < nw) {
-            words[i] = r < rows ? attn_seen_word(a, s.r, attn_token(a, s.row0 + r), w) : 0u;
-          }
-        }
-        if (tid < kRows) {
-          const int row = min(s.row0 + tid, s.r.rows - 1), t = attn_token(a, row);
-          ref[tid] = kAttnUnseen;
-          row_id[tid] = (t << 16) | (s.head * g + row - t * g);
-        }
-        if (tid == 0) *odd_v = 0;
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-          const int i = tid + u * kSoft, r = i / (kDim / 8), ch = i % (kDim / 8);
-          if (r < full)
-            st_shared_v4u(smem_u32(q_s) + (ch >> 3) * (kRows * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), qv[u].x ^ a.q_flip,
-                          qv[u].y ^ a.q_flip, qv[u].z ^ a.q_flip, qv[u].w ^ a.q_flip);
-        }
-        fence_proxy_async_shared();
-        mbar_arrive(q_full);
+        const uint32_t* words = all_words + (k & 1) * kRows * 9;
+        const int* row_id = row_ids + (k & 1) * kRows;
+        int* odd_v = odd_vs + (k & 1);
+        if (tid < kRows) ref[tid] = kAttnUnseen;
+        if (tid == 0) odd_vs[(k + 1) & 1] = 0;
         bar_named(8, kSoft);
 #pragma unroll
         for (int j = 0; j < kCols; ++j) l[j] = 0.f;
@@ -664,7 +708,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
               seen = 0u;
 #pragma unroll
               for (int k = 0; k < kCols; ++k)
-                if (k < live) seen |= ((words[(c0 + k) * 8 + (j >> 5)] >> (j & 31)) & 1u) << k;
+                if (k < live) seen |= ((words[(c0 + k) * 9 + (j >> 5)] >> (j & 31)) & 1u) << k;
             }
 #pragma unroll
             for (int k = 0; k < kCols; ++k) x[k] = (seen >> k) & 1u ? x[k] * c : kNegInf;
@@ -815,7 +859,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
                   if (!(fabsf(v) < __int_as_float(0x7f800000)))
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
-                      if ((words[(c0 + cc + k) * 8 + (j >> 5)] >> (j & 31)) & 1u) o[k] += v;
+                      if ((words[(c0 + cc + k) * 9 + (j >> 5)] >> (j & 31)) & 1u) o[k] += v;
                 }
               }
               if (whole) {
@@ -837,6 +881,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           }
         }
         tc_fence_before();
+        mbar_arrive(seg_done);
       }
     }
     if (tid == 0) a.cross[blockIdx.x] = cross;

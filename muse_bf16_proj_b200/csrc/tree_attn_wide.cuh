@@ -29,14 +29,14 @@ template <int kDim>
 struct WideShape {
   static constexpr int kRows = 256, kTok = 128;
   static constexpr int kHalves = kDim / 64;
-  static constexpr int kThreads = 64 + 256;
+  static constexpr int kThreads = 64 + 256 + 64;  // producer, UMMA, softmax, row loaders
   static constexpr int kStage = kTok * kDim * 2;
   static constexpr int kQ = 128 * kDim * 2;  // one row tile
-  static constexpr int kNK = kDim == 64 ? 4 : 2, kNV = kNK;
+  static constexpr int kNK = kDim == 64 ? 5 : 2, kNV = kNK;
   static constexpr int kTmem = 512;          // S [128], P [2][64], O [2][kDim]
   static constexpr int kOffV = kNK * kStage, kOffQ = kOffV + kNV * kStage, kOffSmall = kOffQ + 2 * kQ;
-  // mask words [256][9] (the ninth zero), exchange [2][128], scan sums, barriers
-  static constexpr int kSmall = 256 * 9 * 4 + 2 * 128 * 4 + 64 + (2 * kNK + 2 * kNV + 11) * 8 + 64;
+  // mask words [2][256][9] (the ninth zero), row ids [2][256], exchange [2][128], scan sums, segments, barriers
+  static constexpr int kSmall = 2 * 256 * 9 * 4 + 2 * 256 * 4 + 2 * 128 * 4 + 64 + 128 + (2 * kNK + 2 * kNV + 13) * 8 + 64;
   static constexpr int kSmem = 1024 + kOffSmall + kSmall;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -67,12 +67,6 @@ __device__ __forceinline__ void st_global_v8(float* p, const float* v) {
                : "memory");
 }
 
-// 16 bytes from global to shared memory without a register; zeros where `live` is false.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-
 // D (+)= A . B with A [128 x 16] in tensor memory (16-bit pairs), B from shared memory.
 __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
@@ -99,17 +93,18 @@ template <bool kHalf, int kDim>
 __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
     tree_attn_wide_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttnArgs a) {
   using Sh = WideShape<kDim>;
-  using Walk = AttnWalk<Sh::kTok, Sh::kRows>;
   constexpr int kHalves = Sh::kHalves, kNK = Sh::kNK, kNV = Sh::kNV, kTok = Sh::kTok;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_align<1024>(smem_raw);
   uint8_t* ring_k = smem;
   uint8_t* ring_v = smem + Sh::kOffV;
   uint8_t* q_s = smem + Sh::kOffQ;
-  uint32_t* words = reinterpret_cast<uint32_t*>(smem + Sh::kOffSmall);  // [256][9]
-  float* swap = reinterpret_cast<float*>(words + 256 * 9);              // [2][128]
+  uint32_t* all_words = reinterpret_cast<uint32_t*>(smem + Sh::kOffSmall);  // [2][256][9]
+  int* row_ids = reinterpret_cast<int*>(all_words + 2 * 256 * 9);           // [2][256]
+  float* swap = reinterpret_cast<float*>(row_ids + 2 * 256);                // [2][128]
   int* sums = reinterpret_cast<int*>(swap + 256);
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(sums + 16);
+  AttnSeg* segs = reinterpret_cast<AttnSeg*>(sums + 16);                    // [2]
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(segs) + 16;
   uint64_t* k_empty = k_full + kNK;
   uint64_t* v_full = k_empty + kNK;
   uint64_t* v_empty = v_full + kNV;
@@ -118,10 +113,12 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
   uint64_t* pv_done = p_full + 2;    // [2]
   uint64_t* s_read = pv_done + 2;    // 256 arrivals as p_full's
   uint64_t* q_full = s_read + 1;
-  uint64_t* fin = q_full + 1;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* seg_done = q_empty + 1;
+  uint64_t* fin = seg_done + 1;
   int* start = reinterpret_cast<int*>(fin + 1);  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start + 2);
-  int* odd_v = reinterpret_cast<int*>(tmem_slot + 1);
+  int* odd_vs = reinterpret_cast<int*>(tmem_slot + 1);  // [2]
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -131,7 +128,10 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
     for (int i = 0; i < kNV; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 256), mbar_init(&pv_done[i], 1);
     mbar_init(s_read, 256);
-    mbar_init(q_full, 256);
+    mbar_init(q_full, 64);
+    mbar_init(q_empty, 1);
+    mbar_init(seg_done, 256);
+    odd_vs[0] = odd_vs[1] = 0;
     mbar_init(fin, 1);
     fence_mbar_init();
   }
@@ -148,23 +148,21 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
   } else if (warp == 1) {
     // ---- UMMA issue --------------------------------------------------------------------------------
     if (uniform(plan.work)) {
-      Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
-      AttnSeg s;
       constexpr uint32_t kType = (1u << 4) | (8u << 24) | (kHalf ? 0u : ((1u << 7) | (1u << 10)));
       constexpr uint32_t idesc_s = kType | (static_cast<uint32_t>(kTok >> 3) << 17);
       constexpr uint32_t idesc_o = kType | (static_cast<uint32_t>(kDim >> 3) << 17) | (1u << 16);
       constexpr uint64_t k_bits = attn_desc_bits(128, 1024 * kHalves, 16);
       constexpr uint64_t v_bits = attn_desc_bits(128, 1024 * kHalves, kHalves > 1 ? 1024 : 0);
       Ring rk, rv;
-      uint32_t seg_phase = 0, v0 = 0;  // products before this segment
+      uint32_t v0 = 0;  // products before this segment
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrAttnMma)) != 0; };
-      while (ok && uniform(walk.next(a, s))) {
+      for (int k = 0;; ++k) {
+        if (!(ok = wait(q_full, k & 1))) break;
+        const AttnSeg& s = segs[k & 1];
         const int pair = uniform(s.r.rows - s.row0 > 128 ? 1 : 0);
         const int products = uniform((s.i1 - s.i0) << pair);
-        ok = wait(q_full, seg_phase);
-        seg_phase ^= 1u;
-        if (!ok) break;
+        if (products == 0) break;
         tc_fence_after();
         // The first (or only) row tile's product waits for a K tile, the last releases it; V alike.
         auto issue_s = [&](int v) {
@@ -181,12 +179,14 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
                 umma_bf16(tmem, dq + ((h * 128 * 128) >> 4) + 2 * k, dk + ((h * 1024) >> 4) + 2 * k, idesc_s, (h | k) != 0);
             if (tile == pair) umma_commit(&k_empty[rk.slot]);
             umma_commit(&s_full[(v0 + v) & 1u]);
+            if (v + 1 == products) umma_commit(q_empty);
           }
           __syncwarp();
           if (tile == pair) rk.next(kNK);
           return true;
         };
-        ok = issue_s(0);
+        // S holds the last scores of the segment before until they have been read.
+        ok = (k == 0 || wait(s_read, (v0 - 1) & 1u)) && issue_s(0);
         for (int u = 0; ok && u <= products; ++u) {
           if (u + 1 < products) {
             ok = wait(s_read, (v0 + u) & 1u) && issue_s(u + 1);
@@ -211,66 +211,40 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           if (tile == pair) rv.next(kNV);
         }
         v0 += products;
+        if (!ok) break;
       }
       if (elect_one()) umma_commit(fin);
       __syncwarp();
       mbar_wait(fin, 0u, kErrAttnDrain, kWaitLimitNs / 10);  // nothing of the tensor cores is under way past here
     }
     __syncwarp();
+  } else if (warp >= 10) {
+    if (plan.work)
+      attn_load_rows<kTok, Sh::kRows, 128, kDim, 64>(a, plan, static_cast<int>(threadIdx.x) - 320, q_s, segs, all_words, row_ids, q_full,
+                                                     q_empty, seg_done);
   } else {
     // ---- softmax: thread = one row -----------------------------------------------------------------
     const int tid = static_cast<int>(threadIdx.x) - 64, wg = tid >> 7;
     const int quarter = warp & 3, tl = quarter * 32 + lane;  // TMEM lane = row of the row tile
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-    const int g = a.heads / a.kv_heads;
     const float kNegInf = __int_as_float(0xff800000);
     const float c = a.scale_log2;
     AttnCross cross = {};
     if (plan.work) {
-      Walk walk(a, plan.b0, plan.s0, plan.w0, plan.w1);
-      AttnSeg s, next;
       uint32_t v0 = 0, v_slot = 0, v_phase = 0;
       bool ok = true;
-      // Q of a segment: a thread a 16-byte chunk at a time, all of them on their way at once.
-      constexpr int kChunks = kDim / 8;
-      auto q_at = [&](int r, int ch) {
-        return smem_u32(q_s) + (r >> 7) * Sh::kQ + (ch >> 3) * (128 * 128) + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4);
-      };
-      auto q_rows = [&](const AttnSeg& s) { return s.r.rows - s.row0 > 128 ? 256 : 128; };
-      auto load_q = [&](const AttnSeg& s) {
-        const int last = min(Sh::kRows, s.r.rows - s.row0) - 1;
-        for (int i = tid; i < q_rows(s) * kChunks; i += 256) {
-          const int r = i / kChunks, ch = i % kChunks, row = s.row0 + min(r, last), t = attn_token(a, row);
-          cp_async16(q_at(r, ch), a.q + (s.r.first + t) * a.q_token + (s.head * g + row - t * g) * a.q_head + ch * 8, r <= last);
-        }
-      };
-      bool more = walk.next(a, next);
-      if (more) load_q(next);
-      while (ok && more) {
-        s = next;
+      for (int k = 0;; ++k) {
+        ok = mbar_wait(q_full, k & 1, kErrAttnSoftmax);
+        if (bar_any(8, 256, !ok)) break;  // every thread is done with the last segment's arrays, too
+        const AttnSeg s = segs[k & 1];
+        if (s.i1 <= s.i0) break;
         const int rows = min(Sh::kRows, s.r.rows - s.row0);
         const bool pair = rows > 128;
-        const int row = pair ? wg * 128 + tl : tl;                   // this thread's row of the unit
+        const int row = pair ? wg * 128 + tl : tl;  // this thread's row of the unit
         const bool mine = row < rows;
-        const int t = mine ? attn_token(a, s.row0 + row) : 0, h = s.head * g + s.row0 + row - t * g;
-        bar_named(8, 256);  // every thread is done with the last segment's words
-        if (wg == 0 || pair) {
-          const int nw = (s.r.drafted + 31) >> 5;
-          for (int w = 0; w < nw; ++w) words[row * 9 + w] = mine ? attn_seen_word(a, s.r, t, w) : 0u;
-          for (int w = nw; w < 9; ++w) words[row * 9 + w] = 0u;
-        }
-        if (tid == 0) *odd_v = 0;
-        cp_async_wait();
-        if (a.q_flip) {  // a negative scale: this thread's own chunks with the other sign
-          for (int i = tid; i < q_rows(s) * kChunks; i += 256) {
-            const uint32_t at = q_at(i / kChunks, i % kChunks);
-            const uint4 v = ld_shared_v4u(at);
-            st_shared_v4u(at, v.x ^ a.q_flip, v.y ^ a.q_flip, v.z ^ a.q_flip, v.w ^ a.q_flip);
-          }
-        }
-        fence_proxy_async_shared();
-        mbar_arrive(q_full);
-        bar_named(8, 256);
+        const uint32_t* words = all_words + (k & 1) * 256 * 9;
+        int* odd_v = odd_vs + (k & 1);
+        if (tid == 0) odd_vs[(k + 1) & 1] = 0;
 
         // The products of this thread's row tile in the sequence, and its row's running values.
         const int step = pair ? 2 : 1, products = (s.i1 - s.i0) << (pair ? 1 : 0);
@@ -385,8 +359,6 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         v0 += products;
-        more = walk.next(a, next);
-        if (more) load_q(next);  // this segment's products, the readers of Q, are done
         if (!pair) l += swap[(wg ^ 1) * 128 + tl];
         const bool whole = s.i0 == 0 && s.i1 == s.r.tiles;
         const long long slot = (static_cast<long long>(blockIdx.x) * 2 + (s.i0 > 0 ? 0 : 1)) * Sh::kRows + row;
@@ -398,6 +370,7 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int odd = *odd_v;
         // A thread writes its own row.
+        const int id = row_ids[(k & 1) * 256 + row], t = id >> 16, h = id & 0xFFFF;
         const int d0 = pair ? 0 : wg * (kDim / 2), d1 = pair ? kDim : d0 + kDim / 2;
         uint16_t* out = a.out + (s.r.first + t) * a.out_token + h * a.out_head;
         const uint16_t* gate = a.gate ? a.gate + (s.r.first + t) * a.gate_token + h * a.gate_head : nullptr;
@@ -446,6 +419,7 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           }
         }
         tc_fence_before();
+        mbar_arrive(seg_done);
       }
     }
     if (tid == 0) a.cross[blockIdx.x] = cross;
