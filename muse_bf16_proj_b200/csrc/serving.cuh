@@ -102,10 +102,13 @@ int check_attention(const MuseTreeAttention* p) {
   return MUSE_OK;
 }
 
-// Rows of a unit: those that share a kv head, rounded up to a variant; past 64 the rows-as-M kernel's 256.
+// Rows of a unit: those that share a kv head, rounded up to a variant. Tokens-as-M up to 64 rows at dim 128, up to 32 at
+// dim 64; rows-as-M past that. Measured at 16 requests x 20000 tokens, 64 rows, dim 128: 152 us tokens-as-M, 244 rows-as-M
+// (its Q leaves the ring two tiles less); 64 rows, dim 64: 60 us and 39; 24 rows, dim 64: 31 us and 38.
 int attention_rows(const MuseTreeAttention* p) {
   const int64_t rows = static_cast<int64_t>(p->max_draft) * (p->heads / p->kv_heads);
-  return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 64 ? 64 : 256));
+  if (rows <= 32 || (rows <= 64 && p->dim == 128)) return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
+  return rows <= 128 ? 128 : 256;
 }
 
 int attention_tokens(int dim, int rows) {  // cached tokens a tile (AttnShape::kTok, WideShape::kTok)
@@ -144,6 +147,7 @@ int make_cache_map(CUtensorMap* map, const void* base, const MuseTreeAttention* 
 template <bool kHalf, int kDim, int kRows, typename Kern>
 int launch_attention_t(Kern kern, int threads, int smem, const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas,
                        cudaStream_t st) {
+  const int group = a.heads / a.kv_heads, rows = std::min(kRows, a.max_draft > kRows / group ? kRows : a.max_draft * group);
   static bool configured[kMaxDevices] = {};
   int dev;
   if (int rc = current_device(&dev)) return rc;
@@ -154,7 +158,7 @@ int launch_attention_t(Kern kern, int threads, int smem, const CUtensorMap& tmk,
   }
   if (int rc = launch_pdl("tree_attention", kern, dim3(static_cast<unsigned>(ctas)), threads, smem, st, tmk, tmv, a)) return rc;
   return launch_pdl("tree_attention join", muse::tree_attn_join_kernel<kHalf, kDim, kRows>,
-                    dim3(static_cast<unsigned>(ctas), static_cast<unsigned>(kRows / muse::attn_join_rows(kRows))), 256, 0, st, a);
+                    dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((rows - 1) / muse::attn_join_rows(kRows) + 1)), 256, 0, st, a);
 }
 
 template <bool kHalf, int kDim, int kRows>
@@ -163,13 +167,21 @@ int launch_attention(const CUtensorMap& tmk, const CUtensorMap& tmv, const muse:
   return launch_attention_t<kHalf, kDim, kRows>(muse::tree_attn_kernel<kHalf, kDim, kRows>, Sh::kThreads, Sh::kSmem, tmk, tmv, a, ctas, st);
 }
 
+template <bool kHalf, int kDim, int kRows>
+int launch_attention_wide(const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas, cudaStream_t st) {
+  using Sh = muse::WideShape<kDim, kRows>;
+  return launch_attention_t<kHalf, kDim, kRows>(muse::tree_attn_wide_kernel<kHalf, kDim, kRows>, Sh::kThreads, Sh::kSmem, tmk, tmv, a, ctas, st);
+}
+
 template <bool kHalf, int kDim>
 int launch_attention_rows(int rows, const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas, cudaStream_t st) {
   if (rows == 16) return launch_attention<kHalf, kDim, 16>(tmk, tmv, a, ctas, st);
   if (rows == 32) return launch_attention<kHalf, kDim, 32>(tmk, tmv, a, ctas, st);
-  if (rows == 64) return launch_attention<kHalf, kDim, 64>(tmk, tmv, a, ctas, st);
-  using Sh = muse::WideShape<kDim>;
-  return launch_attention_t<kHalf, kDim, Sh::kRows>(muse::tree_attn_wide_kernel<kHalf, kDim>, Sh::kThreads, Sh::kSmem, tmk, tmv, a, ctas, st);
+  if constexpr (kDim == 128) {
+    if (rows == 64) return launch_attention<kHalf, kDim, 64>(tmk, tmv, a, ctas, st);
+  }
+  if (rows == 128) return launch_attention_wide<kHalf, kDim, 128>(tmk, tmv, a, ctas, st);
+  return launch_attention_wide<kHalf, kDim, 256>(tmk, tmv, a, ctas, st);
 }
 
 }  // namespace

@@ -101,7 +101,7 @@ struct AttnShape {
   static constexpr int kTmem = kTmemO + kRows <= 64 ? 64 : (kTmemO + kRows <= 128 ? 128 : (kTmemO + kRows <= 256 ? 256 : 512));
   static constexpr int kOffV = kNK * kStage, kOffQ = kOffV + kNV * kStage, kOffP = kOffQ + kQ, kOffSmall = kOffP + kNP * kP;
   // ref, rescale, 1 / sum [kRows]; row ids [2][kRows]; red [4 kTG][kRows]; mask words [2][kRows][9]; segments; barriers.
-  static constexpr int kSmall = kRows * 4 * 5 + 4 * kTG * kRows * 4 + kRows * 72 + 128 + (2 * kNK + 2 * kNV + 11) * 8 + 64;
+  static constexpr int kSmall = kRows * 4 * 5 + 4 * kTG * kRows * 4 + kRows * 72 + 128 + (2 * kNK + 2 * kNV + 13) * 8 + 64;
   static constexpr int kSmem = 1024 + kOffSmall + kSmall;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -465,7 +465,9 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_al
 
 // The row loader (kLanes threads of their own): for each segment of the run its description, mask words and row ids
 // (two places in turn) and Q, as soon as the last product that reads the segment before's Q is done: while that segment's
-// softmax, second products and end still run (a segment's first scores wait for it no longer than that). q_full tells the others (kLanes arrivals); a segment without tiles ends
+// softmax, second products and end still run (a segment's first scores wait for it no longer than that). q_full and
+// seg_done are two barriers each, by segment parity: their waiters may come a whole segment late, and one barrier's parity
+// would then name the next phase. q_full tells the others (kLanes arrivals); a segment without tiles ends
 // the run. Q is [row tiles of kTile rows][halves][kTile][64 dims] swizzled; `fill` rows of it are written, zeros past the rows.
 template <int kTok, int kRows, int kTile, int kDim, int kLanes>
 __device__ __forceinline__ void attn_load_rows(const AttnArgs& a, const AttnPlan& plan, int me, uint8_t* q_s, AttnSeg* segs, uint32_t* words,
@@ -478,18 +480,9 @@ __device__ __forceinline__ void attn_load_rows(const AttnArgs& a, const AttnPlan
     const bool more = walk.next(a, s);
     if (!more) s.i0 = s.i1 = 0;
     // This place's last user, two segments ago, is done with it.
-    if (k > 1 && !mbar_wait(seg_done, k & 1, kErrAttnLoader)) break;
-    if (me == 0) segs[k & 1] = s;
+    if (k > 1 && !mbar_wait(&seg_done[k & 1], ((k >> 1) - 1) & 1, kErrAttnLoader)) break;
     if (more) {
       const int rows = min(kRows, s.r.rows - s.row0), fill = kTile == kRows ? min(kRows, (rows + 15) & ~15) : (rows > kTile ? kRows : kTile);
-      uint32_t* w = words + (k & 1) * kRows * 9;
-      int* id = row_id + (k & 1) * kRows;
-      const int nw = (s.r.drafted + 31) >> 5;
-      for (int r = me; r < fill; r += kLanes) {
-        const int row = s.row0 + min(r, rows - 1), t = attn_token(a, row);
-        id[r] = (t << 16) | (s.head * g + row - t * g);
-        for (int j = 0; j < 9; ++j) w[r * 9 + j] = j < nw && r < rows ? attn_seen_word(a, s.r, t, j) : 0u;
-      }
       if (k > 0 && !mbar_wait(q_empty, (k - 1) & 1, kErrAttnLoader)) break;
       auto at = [&](int r, int ch) {
         return smem_u32(q_s) + (r / kTile) * (kTile * kDim * 2) + (ch >> 3) * (kTile * 128) + (r & (kTile - 1)) * 128 +
@@ -499,6 +492,15 @@ __device__ __forceinline__ void attn_load_rows(const AttnArgs& a, const AttnPlan
       for (int i = me; i < fill * kChunks; i += kLanes) {
         const int r = i / kChunks, ch = i % kChunks, row = s.row0 + min(r, rows - 1), t = attn_token(a, row);
         cp_async16(at(r, ch), a.q + (s.r.first + t) * a.q_token + (s.head * g + row - t * g) * a.q_head + ch * 8, r < rows);
+      }
+      uint32_t* w = words + (k & 1) * kRows * 9;
+      int* id = row_id + (k & 1) * kRows;
+      const int nw = (s.r.drafted + 31) >> 5;
+      for (int r = me; r < fill; r += kLanes) {
+        const int row = s.row0 + min(r, rows - 1), t = attn_token(a, row);
+        id[r] = (t << 16) | (s.head * g + row - t * g);
+        for (int j = 0; j < nw; ++j) w[r * 9 + j] = r < rows ? attn_seen_word(a, s.r, t, j) : 0u;
+        for (int j = nw; j < 9; ++j) w[r * 9 + j] = 0u;
       }
       cp_async_wait();
       if (a.q_flip) {  // a negative scale: this thread's own chunks with the other sign
@@ -510,7 +512,8 @@ __device__ __forceinline__ void attn_load_rows(const AttnArgs& a, const AttnPlan
       }
       fence_proxy_async_shared();
     }
-    mbar_arrive(q_full);
+    if (me == 0) segs[k & 1] = s;
+    mbar_arrive(&q_full[k & 1]);
     if (!more) break;
   }
 }
@@ -544,9 +547,9 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   // would by then name the next phase.
   uint64_t* pv_done = p_full + 2;
   uint64_t* q_full = pv_done + 2;
-  uint64_t* q_empty = q_full + 1;
+  uint64_t* q_empty = q_full + 2;    // q_full [2], seg_done [2]: by segment parity
   uint64_t* seg_done = q_empty + 1;
-  uint64_t* fin = seg_done + 1;
+  uint64_t* fin = seg_done + 2;
   int* start_b = reinterpret_cast<int*>(fin + 1);  // [2]: the run's first request, and the tiles before it
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start_b + 2);
   int* odd_vs = reinterpret_cast<int*>(tmem_slot + 1);  // [2], by segment: a drafted token has a non-finite V entry
@@ -558,9 +561,8 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     for (int i = 0; i < kNK; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
     for (int i = 0; i < kNV; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], kSoft), mbar_init(&pv_done[i], 1);
-    mbar_init(q_full, 32);
+    for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 32), mbar_init(&seg_done[i], kSoft);
     mbar_init(q_empty, 1);
-    mbar_init(seg_done, kSoft);
     odd_vs[0] = odd_vs[1] = 0;
     mbar_init(fin, 1);
     fence_mbar_init();
@@ -612,7 +614,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         return true;
       };
       for (int k = 0;; ++k) {
-        if (!(ok = wait(q_full, k & 1))) break;
+        if (!(ok = wait(&q_full[k & 1], (k >> 1) & 1))) break;
         const int tiles = uniform(segs[k & 1].i1 - segs[k & 1].i0);
         if (tiles == 0) break;
         tc_fence_after();
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       float l[kCols];
       for (int k = 0;; ++k) {
         // ---- the segment's rows --------------------------------------------------------------------
-        ok = mbar_wait(q_full, k & 1, kErrAttnSoftmax);
+        ok = mbar_wait(&q_full[k & 1], (k >> 1) & 1, kErrAttnSoftmax);
         if (bar_any(8, kSoft, !ok)) break;  // every thread is done with the last segment's arrays, too
         const AttnSeg s = segs[k & 1];
         if (s.i1 <= s.i0) break;
@@ -881,7 +883,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           }
         }
         tc_fence_before();
-        mbar_arrive(seg_done);
+        mbar_arrive(&seg_done[k & 1]);
       }
     }
     if (tid == 0) a.cross[blockIdx.x] = cross;
@@ -896,8 +898,9 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
 __host__ __device__ constexpr int attn_join_rows(int rows) { return rows >= 128 ? 8 : rows / 16; }  // rows a CTA
 
 // Joins the partials of the row tiles that cross runs: grid (runs, parts of the rows), 8 warps, of which each
-// row has 8 (16 rows) to 1 (128 and more) that take the runs in turn. Partials are weighed by
-// 2^(their reference - the largest) and added in a fixed order.
+// row has 8 (16 rows) to 1 (128 and more) that take the runs in turn, four partials on their way at once. A
+// partial weighs 2^(its reference - the largest); the order of the sums is fixed. Latency is its cost: one load of
+// what crosses here, then everything else together.
 template <bool kHalf, int kDim, int kRows>
 __global__ void __launch_bounds__(256) tree_attn_join_kernel(const AttnArgs a) {
   constexpr int kN = kDim / 32, kBlock = attn_join_rows(kRows), kPerRow = 8 / kBlock;
@@ -910,58 +913,87 @@ __global__ void __launch_bounds__(256) tree_attn_join_kernel(const AttnArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % kPerRow, col = r0 + warp / kPerRow;
   const int c0 = blockIdx.x, n = x.last - c0 + 1;
   const bool live = col < x.rows;
-  // Run c0 holds the tile's beginning in its second partial, the others their share in their first.
-  auto slot = [&](int k) { return static_cast<long long>((c0 + k) * 2 + (k == 0 ? 1 : 0)) * kRows + col; };
-  float top = kAttnUnseen;
-  if (live)
-    for (int k = lane; k < n; k += 32) top = fmaxf(top, a.part_ml[slot(k)].x);
+  const int row = x.row0 + col, t = attn_token(a, row), g = a.heads / a.kv_heads;
+  const long long token = x.first + t, h = x.head * g + row - t * g;
+  uint32_t gw[kN / 2] = {};
+  if (a.gate && live) {
 #pragma unroll
-  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  float acc[kN], sum = 0.f;
+    for (int i = 0; i < kN / 2; ++i)
+      gw[i] = __ldg(reinterpret_cast<const uint32_t*>(a.gate + token * a.gate_token + h * a.gate_head + lane * kN) + i);
+  }
+  float acc[kN], sum = 0.f, top = kAttnUnseen;
 #pragma unroll
   for (int i = 0; i < kN; ++i) acc[i] = 0.f;
   if (live) {
-#pragma unroll 8
-    for (int k = part; k < n; k += kPerRow) {
-      const float2 ml = a.part_ml[slot(k)];
-      const float* src = a.part_o + slot(k) * kDim + lane * kN;
-      const float w = ex2(ml.x - top);  // 0 for a partial that saw nothing beside one that saw something
-      sum += ml.y * w;
-      if constexpr (kN == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src);
-        acc[0] += w * v.x, acc[1] += w * v.y, acc[2] += w * v.z, acc[3] += w * v.w;
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(src);
-        acc[0] += w * v.x, acc[1] += w * v.y;
+    for (int k0 = part; k0 < n; k0 += 4 * kPerRow) {
+      float2 ml[4];
+      float o[4][kN];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int k = k0 + u * kPerRow;
+        ml[u] = make_float2(kAttnUnseen, 0.f);
+#pragma unroll
+        for (int i = 0; i < kN; ++i) o[u][i] = 0.f;
+        if (k < n) {
+          // Run c0 holds the tile's beginning in its second partial, the others their share in their first.
+          const long long slot = static_cast<long long>((c0 + k) * 2 + (k == 0 ? 1 : 0)) * kRows + col;
+          ml[u] = a.part_ml[slot];
+          const float* src = a.part_o + slot * kDim + lane * kN;
+          if constexpr (kN == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(src);
+            o[u][0] = v.x, o[u][1] = v.y, o[u][2] = v.z, o[u][3] = v.w;
+          } else {
+            const float2 v = *reinterpret_cast<const float2*>(src);
+            o[u][0] = v.x, o[u][1] = v.y;
+          }
+        }
+      }
+      const float now = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), top), f = ex2(top - now);
+      top = now;
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) acc[i] *= f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float w = ex2(ml[u].x - now);
+        sum += ml[u].y * w;
+#pragma unroll
+        for (int i = 0; i < kN; ++i) acc[i] += w * o[u][i];
       }
     }
   }
   if constexpr (kPerRow > 1) {
 #pragma unroll
     for (int i = 0; i < kN; ++i) sums[warp][lane * kN + i] = acc[i];
-    if (lane == 0) sums[warp][kDim] = sum;
+    if (lane == 0) sums[warp][kDim] = sum, sums[warp][kDim + 1] = top;
     __syncthreads();
     if (part != 0) return;
-    for (int w = 1; w < kPerRow; ++w) {
+    float now = top;
 #pragma unroll
-      for (int i = 0; i < kN; ++i) acc[i] += sums[warp + w][lane * kN + i];
-      sum += sums[warp + w][kDim];
+    for (int w = 1; w < kPerRow; ++w) now = fmaxf(now, sums[warp + w][kDim + 1]);
+    const float f = ex2(top - now);
+    sum *= f;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) acc[i] *= f;
+#pragma unroll
+    for (int w = 1; w < kPerRow; ++w) {
+      const float fw = ex2(sums[warp + w][kDim + 1] - now);
+#pragma unroll
+      for (int i = 0; i < kN; ++i) acc[i] += fw * sums[warp + w][lane * kN + i];
+      sum += fw * sums[warp + w][kDim];
     }
   }
   if (!live) return;
-  const int row = x.row0 + col, t = attn_token(a, row), g = a.heads / a.kv_heads;
-  const long long token = x.first + t, h = x.head * g + row - t * g;
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint32_t packed[kN / 2];
 #pragma unroll
-  for (int i = 0; i < kN; i += 2) {
-    float v[2] = {acc[i] * inv, acc[i + 1] * inv};
+  for (int i = 0; i < kN / 2; ++i) {
+    float v[2] = {acc[2 * i] * inv, acc[2 * i + 1] * inv};
     if (a.gate) {
-      const uint32_t gw = *reinterpret_cast<const uint32_t*>(a.gate + token * a.gate_token + h * a.gate_head + lane * kN + i);
-      v[0] = __fdividef(v[0], 1.f + __expf(-lo16<kHalf>(gw)));
-      v[1] = __fdividef(v[1], 1.f + __expf(-hi16<kHalf>(gw)));
+      v[0] = __fdividef(v[0], 1.f + __expf(-lo16<kHalf>(gw[i])));
+      v[1] = __fdividef(v[1], 1.f + __expf(-hi16<kHalf>(gw[i])));
     }
-    packed[i / 2] = pack16x2<kHalf>(v[0], v[1]);
+    packed[i] = pack16x2<kHalf>(v[0], v[1]);
   }
   uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + token * a.out_token + h * a.out_head + lane * kN);
   if constexpr (kN == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(packed[0], packed[1]);

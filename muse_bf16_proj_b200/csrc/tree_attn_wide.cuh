@@ -25,18 +25,19 @@
 
 namespace muse {
 
-template <int kDim>
+// kRows: 256, or 128 where no request has more (one row tile: Q's second place goes to the ring).
+template <int kDim, int kRows_>
 struct WideShape {
-  static constexpr int kRows = 256, kTok = 128;
+  static constexpr int kRows = kRows_, kTok = 128;
   static constexpr int kHalves = kDim / 64;
   static constexpr int kThreads = 64 + 256 + 64;  // producer, UMMA, softmax, row loaders
   static constexpr int kStage = kTok * kDim * 2;
   static constexpr int kQ = 128 * kDim * 2;  // one row tile
-  static constexpr int kNK = kDim == 64 ? 5 : 2, kNV = kNK;
+  static constexpr int kNK = kDim == 64 ? 5 : (kRows == 128 ? 3 : 2), kNV = kDim == 64 ? 5 : (kRows == 128 ? 2 : 2);
   static constexpr int kTmem = 512;          // S [128], P [2][64], O [2][kDim]
-  static constexpr int kOffV = kNK * kStage, kOffQ = kOffV + kNV * kStage, kOffSmall = kOffQ + 2 * kQ;
-  // mask words [2][256][9] (the ninth zero), row ids [2][256], exchange [2][128], scan sums, segments, barriers
-  static constexpr int kSmall = 2 * 256 * 9 * 4 + 2 * 256 * 4 + 2 * 128 * 4 + 64 + 128 + (2 * kNK + 2 * kNV + 13) * 8 + 64;
+  static constexpr int kOffV = kNK * kStage, kOffQ = kOffV + kNV * kStage, kOffSmall = kOffQ + kRows / 128 * kQ;
+  // mask words [2][kRows][9] (the ninth zero), row ids [2][kRows], exchange [2][128], scan sums, segments, barriers
+  static constexpr int kSmall = 2 * kRows * 9 * 4 + 2 * kRows * 4 + 2 * 128 * 4 + 64 + 128 + (2 * kNK + 2 * kNV + 15) * 8 + 64;
   static constexpr int kSmem = 1024 + kOffSmall + kSmall;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -89,19 +90,19 @@ __device__ __forceinline__ uint32_t wide_seen(const uint32_t* row_words, int j0)
   return __funnelshift_r(row_words[j0 >> 5], row_words[(j0 >> 5) + 1], j0 & 31);
 }
 
-template <bool kHalf, int kDim>
-__global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
+template <bool kHalf, int kDim, int kRows>
+__global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
     tree_attn_wide_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttnArgs a) {
-  using Sh = WideShape<kDim>;
+  using Sh = WideShape<kDim, kRows>;
   constexpr int kHalves = Sh::kHalves, kNK = Sh::kNK, kNV = Sh::kNV, kTok = Sh::kTok;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_align<1024>(smem_raw);
   uint8_t* ring_k = smem;
   uint8_t* ring_v = smem + Sh::kOffV;
   uint8_t* q_s = smem + Sh::kOffQ;
-  uint32_t* all_words = reinterpret_cast<uint32_t*>(smem + Sh::kOffSmall);  // [2][256][9]
-  int* row_ids = reinterpret_cast<int*>(all_words + 2 * 256 * 9);           // [2][256]
-  float* swap = reinterpret_cast<float*>(row_ids + 2 * 256);                // [2][128]
+  uint32_t* all_words = reinterpret_cast<uint32_t*>(smem + Sh::kOffSmall);  // [2][kRows][9]
+  int* row_ids = reinterpret_cast<int*>(all_words + 2 * kRows * 9);         // [2][kRows]
+  float* swap = reinterpret_cast<float*>(row_ids + 2 * kRows);              // [2][128]
   int* sums = reinterpret_cast<int*>(swap + 256);
   AttnSeg* segs = reinterpret_cast<AttnSeg*>(sums + 16);                    // [2]
   uint64_t* k_full = reinterpret_cast<uint64_t*>(segs) + 16;
@@ -113,9 +114,9 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
   uint64_t* pv_done = p_full + 2;    // [2]
   uint64_t* s_read = pv_done + 2;    // 256 arrivals as p_full's
   uint64_t* q_full = s_read + 1;
-  uint64_t* q_empty = q_full + 1;
+  uint64_t* q_empty = q_full + 2;    // q_full [2], seg_done [2]: by segment parity
   uint64_t* seg_done = q_empty + 1;
-  uint64_t* fin = seg_done + 1;
+  uint64_t* fin = seg_done + 2;
   int* start = reinterpret_cast<int*>(fin + 1);  // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(start + 2);
   int* odd_vs = reinterpret_cast<int*>(tmem_slot + 1);  // [2]
@@ -128,9 +129,8 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
     for (int i = 0; i < kNV; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1);
     for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 256), mbar_init(&pv_done[i], 1);
     mbar_init(s_read, 256);
-    mbar_init(q_full, 64);
+    for (int i = 0; i < 2; ++i) mbar_init(&q_full[i], 64), mbar_init(&seg_done[i], 256);
     mbar_init(q_empty, 1);
-    mbar_init(seg_done, 256);
     odd_vs[0] = odd_vs[1] = 0;
     mbar_init(fin, 1);
     fence_mbar_init();
@@ -138,13 +138,13 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
   if (warp == 1) tmem_alloc(tmem_slot, Sh::kTmem);
   pdl_launch_dependents();
   pdl_wait();
-  const AttnPlan plan = attn_plan<Sh::kThreads, kTok, Sh::kRows>(a, sums, start);
+  const AttnPlan plan = attn_plan<Sh::kThreads, kTok, kRows>(a, sums, start);
   const uint32_t tmem = static_cast<uint32_t>(uniform(static_cast<int>(*tmem_slot)));
   const uint32_t tmem_p = tmem + 128, tmem_o = tmem + 256;
 
   if (warp == 0) {
     if (plan.work)
-      attn_produce<kTok, Sh::kRows, kDim, kNK, kNV>(a, plan, &tmk, &tmv, ring_k, ring_v, k_full, k_empty, v_full, v_empty);
+      attn_produce<kTok, kRows, kDim, kNK, kNV>(a, plan, &tmk, &tmv, ring_k, ring_v, k_full, k_empty, v_full, v_empty);
   } else if (warp == 1) {
     // ---- UMMA issue --------------------------------------------------------------------------------
     if (uniform(plan.work)) {
@@ -158,9 +158,9 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrAttnMma)) != 0; };
       for (int k = 0;; ++k) {
-        if (!(ok = wait(q_full, k & 1))) break;
+        if (!(ok = wait(&q_full[k & 1], (k >> 1) & 1))) break;
         const AttnSeg& s = segs[k & 1];
-        const int pair = uniform(s.r.rows - s.row0 > 128 ? 1 : 0);
+        const int pair = kRows > 128 ? uniform(s.r.rows - s.row0 > 128 ? 1 : 0) : 0;
         const int products = uniform((s.i1 - s.i0) << pair);
         if (products == 0) break;
         tc_fence_after();
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
     __syncwarp();
   } else if (warp >= 10) {
     if (plan.work)
-      attn_load_rows<kTok, Sh::kRows, 128, kDim, 64>(a, plan, static_cast<int>(threadIdx.x) - 320, q_s, segs, all_words, row_ids, q_full,
+      attn_load_rows<kTok, kRows, 128, kDim, 64>(a, plan, static_cast<int>(threadIdx.x) - 320, q_s, segs, all_words, row_ids, q_full,
                                                      q_empty, seg_done);
   } else {
     // ---- softmax: thread = one row -----------------------------------------------------------------
@@ -234,15 +234,15 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
       uint32_t v0 = 0, v_slot = 0, v_phase = 0;
       bool ok = true;
       for (int k = 0;; ++k) {
-        ok = mbar_wait(q_full, k & 1, kErrAttnSoftmax);
+        ok = mbar_wait(&q_full[k & 1], (k >> 1) & 1, kErrAttnSoftmax);
         if (bar_any(8, 256, !ok)) break;  // every thread is done with the last segment's arrays, too
         const AttnSeg s = segs[k & 1];
         if (s.i1 <= s.i0) break;
-        const int rows = min(Sh::kRows, s.r.rows - s.row0);
-        const bool pair = rows > 128;
+        const int rows = min(kRows, s.r.rows - s.row0);
+        const bool pair = kRows > 128 && rows > 128;
         const int row = pair ? wg * 128 + tl : tl;  // this thread's row of the unit
         const bool mine = row < rows;
-        const uint32_t* words = all_words + (k & 1) * 256 * 9;
+        const uint32_t* words = all_words + (k & 1) * kRows * 9;
         int* odd_v = odd_vs + (k & 1);
         if (tid == 0) odd_vs[(k + 1) & 1] = 0;
 
@@ -261,6 +261,8 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           if (wg == 0 && edge) {
             const bool ragged = (i + 1) * kTok > s.r.kv, drafted = s.r.drafted > 1;
             if (ragged || drafted) {
+              // The place's fill before is complete once PV of two products ago is: only then does the parity name this fill.
+              if (v >= 2) ok = mbar_wait(&pv_done[buffer], ((n - 2) >> 1) & 1u, kErrAttnSoftmax) && ok;
               ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
               const int pos = i * kTok + tl;
               attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), tl, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
         v0 += products;
         if (!pair) l += swap[(wg ^ 1) * 128 + tl];
         const bool whole = s.i0 == 0 && s.i1 == s.r.tiles;
-        const long long slot = (static_cast<long long>(blockIdx.x) * 2 + (s.i0 > 0 ? 0 : 1)) * Sh::kRows + row;
+        const long long slot = (static_cast<long long>(blockIdx.x) * 2 + (s.i0 > 0 ? 0 : 1)) * kRows + row;
         if (!whole && mine && (pair || wg == 0)) a.part_ml[slot] = make_float2(ref, l);
         if (!whole && s.i0 == 0) {
           cross.first = s.r.first, cross.row0 = s.row0, cross.rows = rows, cross.head = s.head;
@@ -370,7 +372,7 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
         const float inv = l == 0.f ? 0.f : 1.f / l;
         const int odd = *odd_v;
         // A thread writes its own row.
-        const int id = row_ids[(k & 1) * 256 + row], t = id >> 16, h = id & 0xFFFF;
+        const int id = row_ids[(k & 1) * kRows + row], t = id >> 16, h = id & 0xFFFF;
         const int d0 = pair ? 0 : wg * (kDim / 2), d1 = pair ? kDim : d0 + kDim / 2;
         uint16_t* out = a.out + (s.r.first + t) * a.out_token + h * a.out_head;
         const uint16_t* gate = a.gate ? a.gate + (s.r.first + t) * a.gate_token + h * a.gate_head : nullptr;
@@ -419,7 +421,7 @@ __global__ void __launch_bounds__(WideShape<kDim>::kThreads, 1)
           }
         }
         tc_fence_before();
-        mbar_arrive(seg_done);
+        mbar_arrive(&seg_done[k & 1]);
       }
     }
     if (tid == 0) a.cross[blockIdx.x] = cross;
