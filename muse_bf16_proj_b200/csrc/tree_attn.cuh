@@ -29,8 +29,9 @@
 // that lies inside one CTA's run is finished there. One that crosses runs leaves (max, sum, O^T) FP32 partials in
 // scratch, at most two a CTA, which tree_attn_join_kernel adds in run order: deterministic, no atomics.
 //
-// Warps: 0 producer (a lane a TMA box: boxes of min(page, 128) tokens x 64 dims, so any page size of 8 or more
-// and any page order), 1 UMMA issue, then 4 (8 at kRows = 128) softmax warps of 32 TMEM lanes each.
+// Warps: 0 brings K and V (a lane a TMA box of min(page, tile) tokens: any page size of 8 or more and any page order),
+// 1 issues the UMMAs, then 4 or 8 softmax warps of 32 TMEM lanes each, then the row loader. All but the producer wait
+// asleep (mbar_wait_idle): polling warps take issue slots from those at work (11 x 13: 29.4 us polling, 28.6 asleep).
 //
 // Entries that no row may see: tokens past the request's end are not loaded (or are whatever the page holds)
 // and their V rows are zeroed in shared memory, because 0 x NaN is NaN; drafted tokens, which some rows see and
@@ -468,8 +469,9 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_al
 // softmax, second products and end still run (a segment's first scores wait for it no longer than that). q_full and
 // seg_done are two barriers each, by segment parity: their waiters may come a whole segment late, and one barrier's parity
 // would then name the next phase. q_full tells the others (kLanes arrivals); a segment without tiles ends
-// the run. Q is [row tiles of kTile rows][halves][kTile][64 dims] swizzled; `fill` rows of it are written, zeros past the rows.
-template <int kTok, int kRows, int kTile, int kDim, int kLanes>
+// the run. Q is [row tiles of kTile rows][halves][kTile][64 dims] swizzled; every row that is computed with is written, a
+// multiple of kFill, zeros past the rows (what stood there would have a say in when the references move).
+template <int kTok, int kRows, int kTile, int kFill, int kDim, int kLanes>
 __device__ __forceinline__ void attn_load_rows(const AttnArgs& a, const AttnPlan& plan, int me, uint8_t* q_s, AttnSeg* segs, uint32_t* words,
                                                int* row_id, uint64_t* q_full, uint64_t* q_empty, uint64_t* seg_done) {
   constexpr int kChunks = kDim / 8;
@@ -480,10 +482,10 @@ __device__ __forceinline__ void attn_load_rows(const AttnArgs& a, const AttnPlan
     const bool more = walk.next(a, s);
     if (!more) s.i0 = s.i1 = 0;
     // This place's last user, two segments ago, is done with it.
-    if (k > 1 && !mbar_wait(&seg_done[k & 1], ((k >> 1) - 1) & 1, kErrAttnLoader)) break;
+    if (k > 1 && !mbar_wait_idle(&seg_done[k & 1], ((k >> 1) - 1) & 1, kErrAttnLoader)) break;
     if (more) {
-      const int rows = min(kRows, s.r.rows - s.row0), fill = kTile == kRows ? min(kRows, (rows + 15) & ~15) : (rows > kTile ? kRows : kTile);
-      if (k > 0 && !mbar_wait(q_empty, (k - 1) & 1, kErrAttnLoader)) break;
+      const int rows = min(kRows, s.r.rows - s.row0), fill = min(kRows, (rows + kFill - 1) / kFill * kFill);
+      if (k > 0 && !mbar_wait_idle(q_empty, (k - 1) & 1, kErrAttnLoader)) break;
       auto at = [&](int r, int ch) {
         return smem_u32(q_s) + (r / kTile) * (kTile * kDim * 2) + (ch >> 3) * (kTile * 128) + (r & (kTile - 1)) * 128 +
                (((ch & 7) ^ (r & 7)) << 4);
@@ -591,7 +593,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       Ring rk, rv;
       uint32_t n = 0;
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrAttnMma)) != 0; };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_idle(bar, parity, kErrAttnMma)) != 0; };
       auto issue_s = [&](uint32_t m, bool last) {
         if (!wait(&k_full[rk.slot], rk.phase)) return false;
         tc_fence_after();
@@ -646,7 +648,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     __syncwarp();
   } else if (warp == Sh::kThreads / 32 - 1) {
     if (plan.work)
-      attn_load_rows<kTok, kRows, kRows, kDim, 32>(a, plan, lane, q_s, segs, all_words, row_ids, q_full, q_empty, seg_done);
+      attn_load_rows<kTok, kRows, kRows, 16, kDim, 32>(a, plan, lane, q_s, segs, all_words, row_ids, q_full, q_empty, seg_done);
   } else {
     // ---- softmax: thread = one token of the tile (a TMEM lane of its token group), its group's columns ----
     const int tid = static_cast<int>(threadIdx.x) - 64;
@@ -667,7 +669,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       float l[kCols];
       for (int k = 0;; ++k) {
         // ---- the segment's rows --------------------------------------------------------------------
-        ok = mbar_wait(&q_full[k & 1], (k >> 1) & 1, kErrAttnSoftmax);
+        ok = mbar_wait_idle(&q_full[k & 1], (k >> 1) & 1, kErrAttnSoftmax);
         if (bar_any(8, kSoft, !ok)) break;  // every thread is done with the last segment's arrays, too
         const AttnSeg s = segs[k & 1];
         if (s.i1 <= s.i0) break;
@@ -687,9 +689,9 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         // ---- tiles ---------------------------------------------------------------------------------
         // A wait that gave up is carried to the next barrier reduction: the loop's end has to be the same for all.
         for (int i = s.i0; i < s.i1; ++i, ++n) {
-          ok = mbar_wait(&s_full[n & 1u], (n >> 1) & 1u, kErrAttnSoftmax) && ok;
+          ok = mbar_wait_idle(&s_full[n & 1u], (n >> 1) & 1u, kErrAttnSoftmax) && ok;
           // P's buffer is free, and with two of them PV of two tiles ago is done, once this has passed.
-          if (n >= static_cast<uint32_t>(kNP)) ok = mbar_wait(&pv_done[(n - kNP) & 1u], ((n - kNP) >> 1) & 1u, kErrAttnSoftmax) && ok;
+          if (n >= static_cast<uint32_t>(kNP)) ok = mbar_wait_idle(&pv_done[(n - kNP) & 1u], ((n - kNP) >> 1) & 1u, kErrAttnSoftmax) && ok;
           tc_fence_after();
           float x[kCols];
           const uint32_t ts = tmem + ((n & 1u) * kTG + tg) * kRows + c0 + lanes;
@@ -756,7 +758,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
 #pragma unroll
               for (int j = 0; j < kCols; ++j)
                 if (j < live) l[j] *= rescale[c0 + j];
-              ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax) && ok;
+              ok = mbar_wait_idle(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax) && ok;
               tc_fence_after();
 #pragma unroll
               for (int cc = 0; cc < kCols; cc += 16) {
@@ -797,7 +799,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
             // In the last tile or two of a request.
             const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && s.r.drafted > 1;
             if (ragged || drafted) {
-              ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
+              ok = mbar_wait_idle(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
               attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), token, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);
             }
           }
@@ -814,7 +816,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           warp_fold16<false>(l + cc, lane);
           if (!(lane & 1)) red[(tg * 4 + quarter) * kRows + c0 + cc + (lane >> 1)] = l[cc];
         }
-        if (ok) ok = mbar_wait(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax);
+        if (ok) ok = mbar_wait_idle(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax);
         ok = !bar_any(8, kSoft, !ok);
         if (!ok) break;
         tc_fence_after();

@@ -42,6 +42,94 @@ struct WideShape {
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
+// One tensor's tiles of a run into its ring of kN, a lane a box.
+template <int kTok, int kRows, int kDim, int kN>
+struct WideFeed {
+  static constexpr int kStage = kTok * kDim * 2;
+  const CUtensorMap* map;
+  uint8_t* ring;
+  uint64_t *full, *empty;
+  int combo, box, lane;
+  AttnWalk<kTok, kRows> walk;
+  AttnSeg s;
+  Ring at;
+  int i, issued, page;
+  bool have, more;
+  __device__ __forceinline__ WideFeed(const AttnArgs& a, const AttnPlan& p, const CUtensorMap* map, int combo, uint8_t* ring, uint64_t* full,
+                                      uint64_t* empty)
+      : map(map), ring(ring), full(full), empty(empty), combo(combo), box(min(a.page, kTok)), lane(threadIdx.x & 31),
+        walk(a, p.b0, p.s0, p.w0, p.w1), i(0), issued(0), page(0), have(false) {
+    segment(a);
+  }
+  __device__ __forceinline__ void lookup(const AttnArgs& a) {
+    const int pos = i * kTok + lane * box;
+    have = lane < kTok / box && pos < s.r.kv;
+    page = have ? a.table[s.b * a.table_row + static_cast<unsigned int>(pos) / static_cast<unsigned int>(a.page)] : 0;
+  }
+  __device__ __forceinline__ void segment(const AttnArgs& a) {
+    more = walk.next(a, s);
+    i = s.i0;
+    if (more) lookup(a);
+  }
+  __device__ __forceinline__ bool ready() const { return __all_sync(0xffffffffu, mbar_test(smem_u32(&empty[at.slot]), at.phase ^ 1u)); }
+  // Issues the current tile and moves on (the next tile's page is on its way while its place is waited for).
+  __device__ __forceinline__ void issue(const AttnArgs& a, uint64_t stream, uint64_t keep) {
+    const int now = page, in = ((i * kTok + lane * box) & (a.page - 1)) >> 3;
+    const bool wrong = have && (now < 0 || now >= a.pages);
+    if (wrong) report_error(kErrAttnPage);
+    const uint32_t bytes = static_cast<uint32_t>(__popc(__ballot_sync(0xffffffffu, have))) * static_cast<uint32_t>(box * kDim * 2);
+    if (lane == 0) mbar_expect_tx(&full[at.slot], bytes);
+    __syncwarp();
+    // Tokens that several row tiles read stay in L2; a request's only reader streams them.
+    if (have)
+      tma_load_5d(ring + at.slot * kStage + lane * box * kDim * 2, map, &full[at.slot], in, (wrong ? 0 : now) * combo + s.head,
+                  s.r.rows > kRows ? keep : stream);
+    at.next(kN);
+    ++issued;
+    if (++i < s.i1) lookup(a);
+    else segment(a);
+  }
+  // The copies still under way land before the CTA may end.
+  __device__ __forceinline__ void drain() {
+    for (int n = max(issued - kN, 0); n < issued; ++n)
+      mbar_wait(&full[n % kN], static_cast<uint32_t>((n / kN) & 1), kErrAttnDrain, kWaitLimitNs / 100);
+  }
+};
+
+// The producer warp: K and V tiles in the order K, V, K, V while both have places free, else whichever has. A K tile is
+// needed a whole softmax before its V tile, and with two V places the one-after-the-other order of attn_produce held back
+// the scores that would free them: 242 us at 128 rows, dim 128 and 822 MB, 141 so. (The tokens-as-M kernel, with three
+// places and every tile waiting on HBM, is faster with that order: 59 us at 32 x 4096, 64 so.)
+template <int kTok, int kRows, int kDim, int kNK, int kNV>
+__device__ __forceinline__ void wide_produce(const AttnArgs& a, const AttnPlan& plan, const CUtensorMap* tmk, const CUtensorMap* tmv,
+                                             uint8_t* ring_k, uint8_t* ring_v, uint64_t* k_full, uint64_t* k_empty, uint64_t* v_full,
+                                             uint64_t* v_empty) {
+  static_assert(kTok / 8 <= 32, "a lane a box");
+  WideFeed<kTok, kRows, kDim, kNK> k(a, plan, tmk, a.k_combo, ring_k, k_full, k_empty);
+  WideFeed<kTok, kRows, kDim, kNV> v(a, plan, tmv, a.v_combo, ring_v, v_full, v_empty);
+  const uint64_t stream = policy_evict_first(), keep = policy_evict_normal();
+  unsigned long long since = 0;  // of a wait under way
+  while (v.more) {
+    bool idle = true;
+    if (k.more && k.ready()) k.issue(a, stream, keep), idle = false;
+    if (v.issued < k.issued && v.ready()) v.issue(a, stream, keep), idle = false;
+    if (!idle) {
+      since = 0;
+      continue;
+    }
+    __nanosleep(40);
+    const unsigned long long now = globaltimer();
+    if (since == 0) since = now;
+    if (now - since > kErrPollNs) {
+      const bool late = now - since > kWaitLimitNs;
+      if (late) report_error(kErrAttnProducer);
+      if (__any_sync(0xffffffffu, late || error_raised())) break;
+    }
+  }
+  k.drain();
+  v.drain();
+}
+
 // kN columns of this warp's lanes.
 template <int kN>
 __device__ __forceinline__ void wide_ld(uint32_t taddr, float (&v)[kN]) {
@@ -144,7 +232,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
 
   if (warp == 0) {
     if (plan.work)
-      attn_produce<kTok, kRows, kDim, kNK, kNV>(a, plan, &tmk, &tmv, ring_k, ring_v, k_full, k_empty, v_full, v_empty);
+      wide_produce<kTok, kRows, kDim, kNK, kNV>(a, plan, &tmk, &tmv, ring_k, ring_v, k_full, k_empty, v_full, v_empty);
   } else if (warp == 1) {
     // ---- UMMA issue --------------------------------------------------------------------------------
     if (uniform(plan.work)) {
@@ -156,7 +244,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
       Ring rk, rv;
       uint32_t v0 = 0;  // products before this segment
       bool ok = true;
-      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, kErrAttnMma)) != 0; };
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_idle(bar, parity, kErrAttnMma)) != 0; };
       for (int k = 0;; ++k) {
         if (!(ok = wait(&q_full[k & 1], (k >> 1) & 1))) break;
         const AttnSeg& s = segs[k & 1];
@@ -220,7 +308,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
     __syncwarp();
   } else if (warp >= 10) {
     if (plan.work)
-      attn_load_rows<kTok, kRows, 128, kDim, 64>(a, plan, static_cast<int>(threadIdx.x) - 320, q_s, segs, all_words, row_ids, q_full,
+      attn_load_rows<kTok, kRows, 128, 128, kDim, 64>(a, plan, static_cast<int>(threadIdx.x) - 320, q_s, segs, all_words, row_ids, q_full,
                                                      q_empty, seg_done);
   } else {
     // ---- softmax: thread = one row -----------------------------------------------------------------
@@ -234,7 +322,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
       uint32_t v0 = 0, v_slot = 0, v_phase = 0;
       bool ok = true;
       for (int k = 0;; ++k) {
-        ok = mbar_wait(&q_full[k & 1], (k >> 1) & 1, kErrAttnSoftmax);
+        ok = mbar_wait_idle(&q_full[k & 1], (k >> 1) & 1, kErrAttnSoftmax);
         if (bar_any(8, 256, !ok)) break;  // every thread is done with the last segment's arrays, too
         const AttnSeg s = segs[k & 1];
         if (s.i1 <= s.i0) break;
@@ -262,14 +350,14 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
             const bool ragged = (i + 1) * kTok > s.r.kv, drafted = s.r.drafted > 1;
             if (ragged || drafted) {
               // The place's fill before is complete once PV of two products ago is: only then does the parity name this fill.
-              if (v >= 2) ok = mbar_wait(&pv_done[buffer], ((n - 2) >> 1) & 1u, kErrAttnSoftmax) && ok;
-              ok = mbar_wait(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
+              if (v >= 2) ok = mbar_wait_idle(&pv_done[buffer], ((n - 2) >> 1) & 1u, kErrAttnSoftmax) && ok;
+              ok = mbar_wait_idle(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
               const int pos = i * kTok + tl;
               attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), tl, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);
               fence_proxy_async_shared();
             }
           }
-          ok = mbar_wait(&s_full[buffer], (n >> 1) & 1u, kErrAttnSoftmax) && ok;
+          ok = mbar_wait_idle(&s_full[buffer], (n >> 1) & 1u, kErrAttnSoftmax) && ok;
           tc_fence_after();
           float x[kN];
           wide_ld<kN>(tmem + col0 + lanes, x);
@@ -303,7 +391,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
             l *= f;
             if (v >= step) {
               // O has to be whole up to this row tile's product before.
-              ok = mbar_wait(&pv_done[(n - step) & 1u], ((n - step) >> 1) & 1u, kErrAttnSoftmax) && ok;
+              ok = mbar_wait_idle(&pv_done[(n - step) & 1u], ((n - step) >> 1) & 1u, kErrAttnSoftmax) && ok;
               tc_fence_after();
               const int d0 = kPair ? 0 : wg * (kDim / 2), d1 = kPair ? kDim : d0 + kDim / 2;
 #pragma unroll 1
@@ -318,7 +406,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
             }
           }
           // P, rounded, once its place is free: 32 scores become 16 words.
-          if (v >= 2) ok = mbar_wait(&pv_done[buffer], ((n - 2) >> 1) & 1u, kErrAttnSoftmax) && ok;
+          if (v >= 2) ok = mbar_wait_idle(&pv_done[buffer], ((n - 2) >> 1) & 1u, kErrAttnSoftmax) && ok;
           tc_fence_after();
           float2 sum = {0.f, 0.f};
           const float2 cc2 = {c, c}, mm2 = {-ref, -ref};
@@ -354,7 +442,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
         // ---- end of the segment: finish the rows, or leave a partial ---------------------------------
         if (ok) {
           const uint32_t n = v0 + products - (pair ? 2 - wg : 1);
-          ok = mbar_wait(&pv_done[n & 1u], (n >> 1) & 1u, kErrAttnSoftmax);
+          ok = mbar_wait_idle(&pv_done[n & 1u], (n >> 1) & 1u, kErrAttnSoftmax);
         }
         swap[wg * 128 + tl] = l;
         ok = !bar_any(8, 256, !ok);

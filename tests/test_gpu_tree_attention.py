@@ -224,6 +224,19 @@ def test_same_bits_again_on_another_stream_and_in_a_graph():
     assert ((got.double() - out).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("drafts,d", [([22, 22], 64), ([11, 9, 10], 128), ([1, 1], 128), ([3, 4], 64), ([7, 30], 128)])
+def test_same_bits_whatever_ran_before(drafts, d):
+    """Rows that a row tile has and the request does not, and what other kernels left in shared and tensor memory,
+    have no say in a result."""
+    a = make([3000 - 700 * b for b in range(len(drafts))], drafts, 12, 4, d, 64, torch.bfloat16)
+    other = make([900, 30], [5, 40], 8, 2, 192 - d, 16, torch.bfloat16, spread=30.0)
+    x = torch.randn((2048, 2048), device="cuda").bfloat16()
+    first = tree_attention(**a)
+    for before in (lambda: tree_attention(**a), lambda: tree_attention(**other), lambda: x @ x, lambda: x.zero_()):
+        before()
+        assert torch.equal(tree_attention(**a), first)
+
+
 def test_offsets_past_32_bits():
     pages, page, hk, d = 33000, 128, 8, 128
     kp = torch.empty((pages, hk, page, d), dtype=torch.bfloat16, device="cuda")
