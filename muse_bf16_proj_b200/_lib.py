@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import re
+import struct
 
 from .build import LIB
 
@@ -382,19 +383,30 @@ def proj_bf16_rows(x_ptr: int, wrows_ptr: int, y_ptr: int, m: int, n: int, k: in
     check(load().muse_proj_bf16_rows(x_ptr, wrows_ptr, y_ptr, m, n, k, ctypes.byref(plan), ctypes.c_void_p(stream)))
 
 
-def rope_append(args: MuseRopeAppend, stream: int) -> None:
-    check(load().muse_rope_append(args, stream))
+# The same structures as packed bytes: a fraction of a ctypes structure's time to fill.
+PACK_ROPE_APPEND = struct.Struct("@9Q16q8i").pack
+PACK_TREE_ATTENTION = struct.Struct("@10Q16q10if4x").pack
+PACK_ROUTE = struct.Struct("@4Qq8if4x").pack
 
 
-def tree_attention(args: MuseTreeAttention, stream: int) -> None:
-    check(load().muse_tree_attention(args, stream))
+def _entry(name: str):
+    """A C entry that takes packed bytes, bound on first use."""
+    bound = None
+
+    def call(packed: bytes, stream: int) -> None:
+        nonlocal bound
+        if bound is None:
+            bound = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)((name, load()))
+        rc = bound(packed, stream)
+        if rc:
+            check(rc)
+    return call
+
+
+rope_append, tree_attention, route = (_entry(f"muse_{op}") for op in ("rope_append", "tree_attention", "route"))
 
 
 def tree_attention_scratch_bytes(args: MuseTreeAttention) -> int:
     out = ctypes.c_int64()
     check(load().muse_tree_attention_scratch_bytes(args, ctypes.byref(out)))
     return out.value
-
-
-def route(args: MuseRoute, stream: int) -> None:
-    check(load().muse_route(args, stream))

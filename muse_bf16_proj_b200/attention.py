@@ -19,6 +19,7 @@ its range is found on the device and recorded in the device error word (``_lib.d
 
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -115,41 +116,57 @@ def tree_mask(parents: torch.Tensor, starts: torch.Tensor, max_draft: int) -> to
     return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).int()
 
 
-def _check_rows(name: str, t: torch.Tensor, device, dtype, dim: int) -> None:
-    if t.dim() != 3 or t.dtype != dtype or t.device != device or t.shape[2] != dim or t.stride(2) != 1:
-        raise ValueError(f"{name}: expected [tokens, heads, {dim}] {dtype} on {device} with contiguous rows, got "
-                         f"{tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
+def _bad(name: str, wanted: str, t: torch.Tensor) -> ValueError:
+    return ValueError(f"{name}: expected {wanted}, got {tuple(t.shape)} {t.dtype} on {t.device} with strides {t.stride()}")
 
 
-def _check_cache(k_pages: torch.Tensor, v_pages: torch.Tensor, device, dtype, kv_heads: int | None, dim: int):
-    shape = k_pages.shape
-    if (k_pages.dim() != 4 or v_pages.shape != shape or shape[3] != dim or (kv_heads is not None and shape[1] != kv_heads) or
-            k_pages.dtype != dtype or v_pages.dtype != dtype or k_pages.device != device or v_pages.device != device or
-            k_pages.stride(3) != 1 or v_pages.stride(3) != 1):
-        raise ValueError(f"k_pages, v_pages: expected [pages, {kv_heads if kv_heads is not None else 'kv_heads'}, page_size, {dim}] "
-                         f"{dtype} on {device}, got {tuple(shape)} {k_pages.dtype} on {k_pages.device} and "
-                         f"{tuple(v_pages.shape)} {v_pages.dtype} on {v_pages.device}")
-    return shape
+# The checks below ask each tensor for each property once (a call is a few microseconds of host time, as much as a
+# small launch) and hand back the strides, which the kernels want too. Devices are compared by index: -1 is the CPU.
 
 
-def _check_vector(name: str, t: torch.Tensor, device, dtype, n: int) -> None:
-    if t.dim() != 1 or t.shape[0] != n or t.dtype != dtype or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected contiguous [{n}] {dtype} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _rows(name: str, t: torch.Tensor, dev: int, dtype, m: int, heads: int, dim: int) -> tuple:
+    stride = t.stride()
+    if t.shape != (m, heads, dim) or t.dtype != dtype or t.get_device() != dev or stride[2] != 1:
+        raise _bad(name, f"[{m}, {heads}, {dim}] {dtype} on device {dev} with contiguous rows", t)
+    return stride
 
 
-def _check_cuda(device: torch.device) -> None:
-    if device.type != "cuda":
-        raise ValueError(f"expected CUDA tensors, got {device}")
+def _cache(k_pages: torch.Tensor, v_pages: torch.Tensor, dev: int, dtype, dim: int):
+    shape, ck, cv = k_pages.shape, k_pages.stride(), v_pages.stride()
+    if (len(shape) != 4 or v_pages.shape != shape or shape[3] != dim or k_pages.dtype != dtype or v_pages.dtype != dtype or
+            k_pages.get_device() != dev or v_pages.get_device() != dev or ck[3] != 1 or cv[3] != 1):
+        raise ValueError(f"k_pages, v_pages: expected two of [pages, kv_heads, page_size, {dim}] {dtype} on device {dev} with contiguous "
+                         f"rows, got {tuple(shape)} {k_pages.dtype} on {k_pages.device} and {tuple(v_pages.shape)} {v_pages.dtype} on "
+                         f"{v_pages.device}")
+    return shape, ck, cv
 
 
-def _on(device: torch.device, call, args) -> None:
-    """``call(args, stream)`` on the tensors' device, which need not be the current one."""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        call(args, stream)
+def _vector(name: str, t: torch.Tensor, dev: int, dtype, n: int) -> int:
+    if t.shape != (n,) or t.dtype != dtype or t.get_device() != dev or (n > 1 and t.stride(0) != 1):
+        raise _bad(name, f"contiguous [{n}] {dtype} on device {dev}", t)
+    return t.data_ptr()
+
+
+def _words(name: str, t: torch.Tensor, dev: int, rows: int) -> int:
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != rows or t.dtype != torch.int32 or t.get_device() != dev or (shape[1] > 1 and t.stride(1) != 1):
+        raise _bad(name, f"[{rows}, columns] int32 on device {dev} with contiguous rows", t)
+    return t.data_ptr()
+
+
+def _check_cuda(t: torch.Tensor, dev: int) -> None:
+    if dev < 0:
+        raise ValueError(f"expected CUDA tensors, got {t.device}")
+
+
+def _call(dev: int, entry, packed: bytes) -> None:
+    """``entry(packed arguments, torch's current stream)`` on the tensors' device, which need not be the current one."""
+    stream = torch._C._cuda_getCurrentRawStream(dev)
+    if dev == torch.cuda.current_device():
+        entry(packed, stream)
     else:
-        with torch.cuda.device(device):
-            call(args, stream)
+        with torch.cuda.device(dev):
+            entry(packed, stream)
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor,
@@ -160,36 +177,27 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     may be q itself, or a new contiguous tensor). BF16 or FP16, D 64 or 128; q, k, v may be strided views of
     one projection output. ``rope``: FP32 [positions, rotary] (``rope_table``); pairs are (i, i + rotary / 2),
     or (2i, 2i + 1) when ``interleaved``; entries past ``rotary`` are left as they are."""
-    device, dtype = q.device, q.dtype
-    if q.dim() != 3 or dtype not in _TYPES:
+    dev, dtype = q.get_device(), q.dtype
+    kind = _TYPES.get(dtype)
+    if q.dim() != 3 or kind is None:
         raise ValueError(f"q: expected [tokens, heads, dim] in bfloat16 or float16, got {tuple(q.shape)} {dtype}")
     m, heads, dim = q.shape
-    _check_rows("q", q, device, dtype, dim)
-    _check_rows("k", k, device, dtype, dim)
-    _check_rows("v", v, device, dtype, dim)
-    kv_heads = k.shape[1]
-    if k.shape != v.shape or k.shape[0] != m:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} do not go with q {tuple(q.shape)}")
-    pages, _, page_size, _ = _check_cache(k_pages, v_pages, device, dtype, kv_heads, dim)
-    _check_vector("positions", positions, device, torch.int32, m)
-    _check_vector("slots", slots, device, torch.int64, m)
-    if rope.dim() != 2 or rope.dtype != torch.float32 or rope.device != device or not rope.is_contiguous() or rope.shape[1] > dim:
-        raise ValueError(f"rope: expected contiguous [positions, rotary <= {dim}] float32 on {device}, got {tuple(rope.shape)} "
-                         f"{rope.dtype} on {rope.device}")
+    (pages, kv_heads, page_size, _), ck, cv = _cache(k_pages, v_pages, dev, dtype, dim)
+    sq, sk, sv = _rows("q", q, dev, dtype, m, heads, dim), _rows("k", k, dev, dtype, m, kv_heads, dim), _rows("v", v, dev, dtype, m, kv_heads, dim)
+    position, slot = _vector("positions", positions, dev, torch.int32, m), _vector("slots", slots, dev, torch.int64, m)
+    table = rope.shape
+    if len(table) != 2 or table[1] > dim or rope.dtype != torch.float32 or rope.get_device() != dev or not rope.is_contiguous():
+        raise _bad("rope", f"contiguous [positions, rotary <= {dim}] float32 on device {dev}", rope)
     if q_out is not None:
-        _check_rows("q_out", q_out, device, dtype, dim)
-        if q_out.shape != q.shape:
-            raise ValueError(f"q_out {tuple(q_out.shape)} is not q's shape {tuple(q.shape)}")
-    _check_cuda(device)
+        so = _rows("q_out", q_out, dev, dtype, m, heads, dim)
+    _check_cuda(q, dev)
     if q_out is None:
-        q_out = torch.empty((m, heads, dim), dtype=dtype, device=device)
-    sq, sk, sv, so, ck, cv = q.stride(), k.stride(), v.stride(), q_out.stride(), k_pages.stride(), v_pages.stride()
-    args = _lib.MuseRopeAppend(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), rope.data_ptr(),
-        positions.data_ptr(), slots.data_ptr(), sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], so[0], so[1], ck[0], ck[1], ck[2],
-        cv[0], cv[1], cv[2], rope.shape[0], pages, m, heads, kv_heads, dim, rope.shape[1], page_size, interleaved,
-        _TYPES[dtype])
-    _on(device, _lib.rope_append, args)
+        q_out = torch.empty((m, heads, dim), dtype=dtype, device=q.device)
+        so = (heads * dim, dim)
+    _call(dev, _lib.rope_append, _lib.PACK_ROPE_APPEND(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), rope.data_ptr(), position, slot,
+        sq[0], sq[1], sk[0], sk[1], sv[0], sv[1], so[0], so[1], ck[0], ck[1], ck[2], cv[0], cv[1], cv[2], table[0], pages, m, heads, kv_heads,
+        dim, table[1], page_size, interleaved, kind))
     return q_out
 
 
@@ -207,62 +215,44 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     see the function of that name) sets; without a mask itself and every earlier one, so ``max_draft`` 1 is
     plain decoding. ``scale`` is 1 / sqrt(D) by default. ``gate`` [M, Hq, D] multiplies the result by its
     sigmoid. A row that sees nothing is 0. BF16 or FP16, D 64 or 128; q and gate may be strided views."""
-    device, dtype = q.device, q.dtype
-    if q.dim() != 3 or dtype not in _TYPES:
+    dev, dtype = q.get_device(), q.dtype
+    kind = _TYPES.get(dtype)
+    if q.dim() != 3 or kind is None:
         raise ValueError(f"q: expected [tokens, heads, dim] in bfloat16 or float16, got {tuple(q.shape)} {dtype}")
     m, heads, dim = q.shape
-    _check_rows("q", q, device, dtype, dim)
-    pages, kv_heads, page_size, _ = _check_cache(k_pages, v_pages, device, dtype, None, dim)
-    requests = context.shape[0]
-    _check_vector("context", context, device, torch.int32, requests)
-    _check_vector("starts", starts, device, torch.int32, requests + 1)
-    if page_table.dim() != 2 or page_table.shape[0] != requests or page_table.dtype != torch.int32 or page_table.device != device or (
-            page_table.stride(1) != 1 and page_table.shape[1] > 1):
-        raise ValueError(f"page_table: expected [{requests}, pages] int32 on {device} with contiguous rows, got "
-                         f"{tuple(page_table.shape)} {page_table.dtype} on {page_table.device}")
-    mask_ptr = mask_row = words = 0
+    sq = _rows("q", q, dev, dtype, m, heads, dim)
+    (pages, kv_heads, page_size, _), ck, cv = _cache(k_pages, v_pages, dev, dtype, dim)
+    requests = context.shape[0] if context.dim() else 0
+    lengths, first = _vector("context", context, dev, torch.int32, requests), _vector("starts", starts, dev, torch.int32, requests + 1)
+    table = _words("page_table", page_table, dev, requests)
+    mask = mask_row = words = 0
     if tree_mask is not None:
-        if tree_mask.dim() != 2 or tree_mask.shape[0] != m or tree_mask.dtype != torch.int32 or tree_mask.device != device or (
-                tree_mask.stride(1) != 1 and tree_mask.shape[1] > 1):
-            raise ValueError(f"tree_mask: expected [{m}, words] int32 on {device} with contiguous rows, got {tuple(tree_mask.shape)} "
-                             f"{tree_mask.dtype} on {tree_mask.device}")
-        mask_ptr, mask_row, words = tree_mask.data_ptr(), tree_mask.stride(0), tree_mask.shape[1]
-    gate_ptr = gate_token = gate_head = 0
+        mask = _words("tree_mask", tree_mask, dev, m)
+        mask_row, words = tree_mask.stride(0), tree_mask.shape[1]
+    gates, sg = 0, (0, 0)
     if gate is not None:
-        _check_rows("gate", gate, device, dtype, dim)
-        if gate.shape != q.shape:
-            raise ValueError(f"gate {tuple(gate.shape)} is not q's shape {tuple(q.shape)}")
-        gate_ptr, gate_token, gate_head = gate.data_ptr(), gate.stride(0), gate.stride(1)
+        sg = _rows("gate", gate, dev, dtype, m, heads, dim)
+        gates = gate.data_ptr()
     if out is not None:
-        _check_rows("out", out, device, dtype, dim)
-        if out.shape != q.shape:
-            raise ValueError(f"out {tuple(out.shape)} is not q's shape {tuple(q.shape)}")
-    _check_cuda(device)
+        so = _rows("out", out, dev, dtype, m, heads, dim)
+    _check_cuda(q, dev)
     if out is None:
-        out = torch.empty((m, heads, dim), dtype=dtype, device=device)
+        out = torch.empty((m, heads, dim), dtype=dtype, device=q.device)
+        so = (heads * dim, dim)
     if scale is None:
-        scale = 1.0 / math.sqrt(dim)
-    sq, so, ck, cv = q.stride(), out.stride(), k_pages.stride(), v_pages.stride()
-    args = _lib.MuseTreeAttention(
-        q.data_ptr(), gate_ptr, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-        context.data_ptr(), starts.data_ptr(), mask_ptr, 0, 0, sq[0], sq[1], gate_token, gate_head, so[0], so[1], ck[0],
-        ck[1], ck[2], cv[0], cv[1], cv[2], page_table.stride(0), mask_row, pages, m, requests, max_draft,
-        page_table.shape[1], words, heads, kv_heads, dim, page_size, _TYPES[dtype], scale)
-    scratch = torch.empty(_scratch_bytes(args, device), dtype=torch.uint8, device=device)
-    args.scratch, args.scratch_bytes = scratch.data_ptr(), scratch.numel()
-    _on(device, _lib.tree_attention, args)
+        scale = dim ** -0.5
+    need = _scratch_bytes(dev, requests, max_draft, heads, kv_heads, dim)
+    scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _call(dev, _lib.tree_attention, _lib.PACK_TREE_ATTENTION(
+        q.data_ptr(), gates, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table, lengths, first, mask, scratch.data_ptr(), need,
+        sq[0], sq[1], sg[0], sg[1], so[0], so[1], ck[0], ck[1], ck[2], cv[0], cv[1], cv[2], page_table.stride(0), mask_row, pages, m, requests,
+        max_draft, page_table.shape[1], words, heads, kv_heads, dim, page_size, kind, scale))
     return out
 
 
-_scratch_need: dict = {}
-
-
-def _scratch_bytes(args: _lib.MuseTreeAttention, device: torch.device) -> int:
+@functools.lru_cache(maxsize=None)
+def _scratch_bytes(dev: int, requests: int, max_draft: int, heads: int, kv_heads: int, dim: int) -> int:
     """What the split of the cache needs, by the sizes that decide it."""
-    key = (device.index, args.requests, args.max_draft, args.heads, args.kv_heads, args.dim)
-    need = _scratch_need.get(key)
-    if need is None:
-        with torch.cuda.device(device):
-            need = _lib.tree_attention_scratch_bytes(args)
-        _scratch_need[key] = need
-    return need
+    with torch.cuda.device(dev):
+        return _lib.tree_attention_scratch_bytes(_lib.MuseTreeAttention(requests=requests, max_draft=max_draft, heads=heads, kv_heads=kv_heads,
+                                                                        dim=dim, scale=1.0))

@@ -11,7 +11,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .attention import _check_cuda, _on
+from .attention import _call, _check_cuda, _vector
 
 _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
 _SCORINGS = ("softmax", "sigmoid")
@@ -27,25 +27,21 @@ def route(logits: torch.Tensor, top_k: int, *, scoring: str = "softmax", bias: t
     experts are that many equal runs, a group worth its best choice (with a bias: the sum of its best two),
     and only the best ``top_groups`` take part. ``renormalize`` divides the chosen scores by their sum; all are
     multiplied by ``scale``. An expert masked by -inf (or NaN) comes after every other and weighs 0."""
-    if logits.dim() != 2 or logits.dtype not in _TYPES or (logits.stride(1) != 1 and logits.shape[1] > 1):
+    kind = _TYPES.get(logits.dtype)
+    if logits.dim() != 2 or kind is None or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError(f"logits: expected [tokens, experts] in float32, bfloat16 or float16 with contiguous rows, got "
                          f"{tuple(logits.shape)} {logits.dtype} with strides {logits.stride()}")
     if scoring not in _SCORINGS:
         raise ValueError(f"unknown scoring {scoring!r}")
-    device = logits.device
+    dev = logits.get_device()
     m, experts = logits.shape
-    bias_ptr = 0
-    if bias is not None:
-        if bias.dim() != 1 or bias.shape[0] != experts or bias.dtype != torch.float32 or bias.device != device or not bias.is_contiguous():
-            raise ValueError(f"bias: expected contiguous [{experts}] float32 on {device}, got {tuple(bias.shape)} {bias.dtype} on "
-                             f"{bias.device}")
-        bias_ptr = bias.data_ptr()
+    balance = 0 if bias is None else _vector("bias", bias, dev, torch.float32, experts)
     if top_k < 1:
         raise ValueError(f"top_k must be positive (got {top_k})")
-    _check_cuda(device)
+    _check_cuda(logits, dev)
+    device = logits.device
     weights = torch.empty((m, top_k), dtype=torch.float32, device=device)
     ids = torch.empty((m, top_k), dtype=torch.int32, device=device)
-    args = _lib.MuseRoute(logits.data_ptr(), bias_ptr, weights.data_ptr(), ids.data_ptr(), logits.stride(0), m, experts, top_k, groups,
-                          top_groups, scoring == "sigmoid", renormalize, _TYPES[logits.dtype], scale)
-    _on(device, _lib.route, args)
+    _call(dev, _lib.route, _lib.PACK_ROUTE(logits.data_ptr(), balance, weights.data_ptr(), ids.data_ptr(), logits.stride(0), m, experts, top_k,
+                                           groups, top_groups, scoring == "sigmoid", renormalize, kind, scale))
     return weights, ids

@@ -85,6 +85,11 @@ def test_structs_have_the_headers_size():
     assert ctypes.sizeof(_lib.MuseRopeAppend) == 8 * 25 + 4 * 8
     assert ctypes.sizeof(_lib.MuseTreeAttention) == 8 * 26 + 4 * 11 + 4
     assert ctypes.sizeof(_lib.MuseRoute) == 8 * 5 + 4 * 9 + 4
+    # The packed bytes are the structures.
+    for cls, pack in ((_lib.MuseRopeAppend, _lib.PACK_ROPE_APPEND), (_lib.MuseTreeAttention, _lib.PACK_TREE_ATTENTION),
+                      (_lib.MuseRoute, _lib.PACK_ROUTE)):
+        values = [0.5 if t is ctypes.c_float else i + 1 for i, (_, t) in enumerate(cls._fields_)]
+        assert pack(*values) == bytes(cls(*values))
 
 
 def _attention(**kw):
