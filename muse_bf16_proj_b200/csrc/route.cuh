@@ -34,8 +34,9 @@ struct RouteArgs {
   int32_t* experts;   // [tokens, top_k]
   long long row;      // logits row stride in elements
   int tokens, count, top_k, groups, top_groups, group_size;
+  int group_lanes;           // lanes of a group where it is a power of two of lanes, else 0: one group, or scanned in shared memory
   unsigned int group_magic;  // e / group_size = (e * group_magic) >> 20 for e < 1024
-  int sigmoid, renormalize, vector;
+  int sigmoid, renormalize, vector, bias_vector;
   float scale;
 };
 
@@ -80,10 +81,13 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
   float bias[kN];
 #pragma unroll
   for (int j = 0; j < kJ; ++j) {
+    const int e = j * 128 + lane * 4;
+    if (a.bias_vector) {
+      const float4 b = e < a.count ? __ldg(reinterpret_cast<const float4*>(a.bias + e)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      bias[j * 4] = b.x, bias[j * 4 + 1] = b.y, bias[j * 4 + 2] = b.z, bias[j * 4 + 3] = b.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int e = j * 128 + lane * 4 + i;
-      bias[j * 4 + i] = a.bias && e < a.count ? a.bias[e] : 0.f;
+      for (int i = 0; i < 4; ++i) bias[j * 4 + i] = a.bias && e + i < a.count ? __ldg(a.bias + e + i) : 0.f;
     }
   }
   pdl_wait();
@@ -151,7 +155,38 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
     }
   }
 
-  if (a.groups > 1) {
+  if (a.group_lanes > 0) {
+    // A group is 4 x 2^i experts of one 128-block: the lanes that hold it fold their two best by shuffles.
+    float worth[kJ];
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) {
+      uint32_t b1 = max(key[j * 4], key[j * 4 + 1]), b2 = min(key[j * 4], key[j * 4 + 1]);
+      const uint32_t c1 = max(key[j * 4 + 2], key[j * 4 + 3]), c2 = min(key[j * 4 + 2], key[j * 4 + 3]);
+      b2 = max(max(b2, c2), min(b1, c1));
+      b1 = max(b1, c1);
+      for (int o = a.group_lanes >> 1; o; o >>= 1) {
+        const uint32_t d1 = __shfl_xor_sync(0xffffffffu, b1, o), d2 = __shfl_xor_sync(0xffffffffu, b2, o);
+        b2 = max(max(b2, d2), min(b1, d1));
+        b1 = max(b1, d1);
+      }
+      worth[j] = a.bias ? key_value(b1) + key_value(b2) : key_value(b1);
+    }
+    // Rank of each held group: groups of a block follow one another over its lanes.
+    const int in_block = 32 / a.group_lanes, mine = lane / a.group_lanes;
+    int rank[kJ] = {};
+#pragma unroll
+    for (int j = 0; j < kJ; ++j) {
+      for (int o = 0; o < in_block; ++o) {
+        if (j * in_block + o >= a.groups) break;
+        const float w = __shfl_sync(0xffffffffu, worth[j], o * a.group_lanes);
+#pragma unroll
+        for (int k = 0; k < kJ; ++k) rank[k] += (w > worth[k]) || (w == worth[k] && (j < k || (j == k && o < mine)));
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kN; ++n)
+      if (rank[n >> 2] >= a.top_groups) key[n] = 0u;
+  } else if (a.groups > 1) {
     // Each group's worth: `per` lanes (a power of two) scan one group from shared memory.
 #pragma unroll
     for (int j = 0; j < kJ; ++j) {
@@ -201,13 +236,25 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
     }
   }
 
-  // Top-k: this lane's best key and its place, refreshed only by the lane that gave the last one.
-  uint32_t best = 0u;
-  int at = 0;
+  // Top-k: this lane's best two keys and their places; on a win the second moves up, and a lane that wins again
+  // (under one a token at k = 8) looks through what it has left.
+  uint32_t best, next, gone = 0u;
+  int at, after;
+  auto look = [&]() {
+    best = next = 0u;
+    at = after = 0;
 #pragma unroll
-  for (int n = 0; n < kN; ++n) {
-    if (key[n] > best) best = key[n], at = n;
-  }
+    for (int n = 0; n < kN; ++n) {
+      const uint32_t k = (gone >> n) & 1u ? 0u : key[n];
+      const bool first = k > best, second = k > next;
+      next = first ? best : (second ? k : next);
+      after = first ? at : (second ? n : after);
+      best = first ? k : best;
+      at = first ? n : at;
+    }
+  };
+  look();
+  bool spare = true;  // `next` is this lane's second best
   int chosen = 0;
   for (int r = 0; r < a.top_k; ++r) {
     const uint32_t m = __reduce_max_sync(0xffffffffu, best);
@@ -215,12 +262,12 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
     const int e = __reduce_min_sync(0xffffffffu, best == m ? mine : 0x7FFFFFFF);
     if (lane == r) chosen = e;
     if (best == m && mine == e) {
-      best = 0u;
-      const int taken = at;
-#pragma unroll
-      for (int n = 0; n < kN; ++n) {
-        if (n == taken) key[n] = 0u;
-        if (key[n] > best) best = key[n], at = n;
+      gone |= 1u << at;
+      if (spare) {
+        best = next, at = after, spare = false;
+      } else {
+        look();
+        spare = true;
       }
     }
   }

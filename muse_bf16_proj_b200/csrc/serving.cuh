@@ -316,9 +316,12 @@ extern "C" int muse_route(const MuseRoute* p, void* stream) {
   a.tokens = p->tokens, a.count = p->experts, a.top_k = p->top_k, a.groups = p->groups, a.top_groups = p->top_groups;
   a.group_size = p->experts / p->groups;
   a.group_magic = (1u << 20) / static_cast<unsigned>(a.group_size) + 1u;
+  const int lanes = a.group_size / 4;
+  a.group_lanes = p->groups > 1 && a.group_size % 4 == 0 && lanes <= 32 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
   a.sigmoid = p->sigmoid ? 1 : 0, a.renormalize = p->renormalize ? 1 : 0;
   // Four logits a load where every lane's four are in one row and aligned together.
   a.vector = p->experts % 4 == 0 && p->row % 4 == 0 && aligned_to(p->logits, static_cast<unsigned>(4 * size));
+  a.bias_vector = p->bias && p->experts % 4 == 0 && aligned16(p->bias);
   a.scale = p->scale;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (p->type == MUSE_F32) return launch_route<muse::kRouteF32>(a, st);
