@@ -7,7 +7,7 @@
 //
 // Bound: bytes (q, k, v in; q and the cache rows out), 16-byte accesses throughout. A thread owns one
 // 16-element piece of a head (eight pairs) and walks heads with it, so its table entries are loaded
-// once a token and stay in registers; a CTA's threads cover 16 (dim 128) or 32 (dim 64) heads at a time.
+// once a token and stay in registers; a CTA covers 8 (dim 128) or 16 (dim 64) heads at a time.
 // Rotary sizes, strides or pointers that rule out 16-byte accesses take the scalar kernel, one pair a
 // thread.
 #pragma once
@@ -20,7 +20,7 @@
 namespace muse {
 
 constexpr unsigned int kErrRopePosition = 0xA01, kErrRopeSlot = 0xA02;
-constexpr int kRopeThreads = 128;
+constexpr int kRopeThreads = 64;  // 4096 tokens x 80 heads of 128: 29.4 us, 31.2 with 128 threads, 36.0 with 256
 
 struct RopeArgs {
   const uint16_t *q, *k, *v;
