@@ -484,17 +484,20 @@ int muse_rope_append(const MuseRopeAppend* args, void* stream);
  * keys and values are already in the cache at entries context[b] + j. Every row sees the context; drafted token
  * j where bit j % 32 of word j / 32 of its mask row is set (mask NULL: its own and every earlier one).
  * out = softmax(scale * q . K) V over what the row sees, 0 where it sees nothing, times sigmoid(gate) if gate is
- * given; FP32 softmax statistics and sums, rounded once. Entries of the cache that a row does not see, and what the
+ * given; FP32 softmax statistics and sums, rounded once (the weights of V to the 16-bit type on the way). Entries of the cache that a row does not see, and what the
  * pages hold past a request's tokens, never reach its result, whatever they hold.
  * `scratch`: muse_tree_attention_scratch_bytes, not initialised, not shared by calls that overlap in time.
  * Device error word: 0xB01 a request with more than max_draft tokens, 0xB02 a request past its page table,
  * 0xB03 a page outside the cache; the requests concerned have unspecified results, the others are right.
+ * Limits: pointers and rows 16-byte aligned; cache strides below 2^35, a page's a multiple of a head's (both orders of
+ * page entries and heads are); table_cols * page_size at most 2^30; requests x kv_heads x tiles of 128 entries x tiles
+ * of 128 rows below 2^31, counted from table_cols and max_draft; scale finite and not 0.
  */
 typedef struct MuseTreeAttention {
   const void* q;            /* [tokens, heads, dim] */
   const void* gate;         /* [tokens, heads, dim] or NULL */
   void* out;                /* [tokens, heads, dim] */
-  const void* k_pages;      /* [pages, kv_heads, page_size, dim], any page, head and entry strides */
+  const void* k_pages;      /* [pages, kv_heads, page_size, dim], strides below */
   const void* v_pages;
   const int32_t* table;     /* [requests, table_cols] page of each page_size entries */
   const int32_t* context;   /* [requests] */
@@ -514,8 +517,8 @@ typedef struct MuseTreeAttention {
 
 int muse_tree_attention(const MuseTreeAttention* args, void* stream);
 
-/* Scratch bytes of a muse_tree_attention call on the current device (reads only requests, max_draft, heads,
- * kv_heads and dim of args). */
+/* Scratch bytes of a muse_tree_attention call on the current device: depends on max_draft, heads, kv_heads and dim alone
+ * (tokens, requests, type and scale of args are checked too; no pointer is read). */
 int muse_tree_attention_scratch_bytes(const MuseTreeAttention* args, int64_t* bytes);
 
 /*

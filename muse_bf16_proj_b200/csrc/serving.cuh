@@ -102,13 +102,14 @@ int check_attention(const MuseTreeAttention* p) {
   return MUSE_OK;
 }
 
-// Rows of a unit: those that share a kv head, rounded up to a variant. Tokens-as-M up to 64 rows at dim 128, up to 32 at
-// dim 64; rows-as-M past that. Measured at 16 requests x 20000 tokens, 64 rows, dim 128: 152 us tokens-as-M, 244 rows-as-M
-// (its Q leaves the ring two tiles less); 64 rows, dim 64: 60 us and 39; 24 rows, dim 64: 31 us and 38.
+// Rows of a unit: those that share a kv head, rounded up to a variant. Tokens-as-M up to 32 rows, rows-as-M past that.
+// Measured, tokens-as-M and rows-as-M, at 1 x 700, 1 x 20000, 8 x 3000 and 16 x 20000 (requests x entries), 8 kv heads of
+// 128: 20 rows 12.1 and 12.6, 22.1 and 25.2, 20.8 and 21.0, 132 and 132 us; 64 rows (a softmax thread a token and 32
+// columns) 14.9 and 13.4, 27.5 and 26.4, 26.9 and 24.4, 142 and 133 us. 2 kv heads of 64: 32 rows 11.9 and 9.7, 14.8 and
+// 20.5, 14.1 and 13.3, 28.9 and 37.2 us.
 int attention_rows(const MuseTreeAttention* p) {
   const int64_t rows = static_cast<int64_t>(p->max_draft) * (p->heads / p->kv_heads);
-  if (rows <= 32 || (rows <= 64 && p->dim == 128)) return rows <= 16 ? 16 : (rows <= 32 ? 32 : 64);
-  return rows <= 128 ? 128 : 256;
+  return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 128 ? 128 : 256));
 }
 
 int attention_tokens(int dim, int rows) {  // cached tokens a tile (AttnShape::kTok, WideShape::kTok)
@@ -177,9 +178,6 @@ template <bool kHalf, int kDim>
 int launch_attention_rows(int rows, const CUtensorMap& tmk, const CUtensorMap& tmv, const muse::AttnArgs& a, int ctas, cudaStream_t st) {
   if (rows == 16) return launch_attention<kHalf, kDim, 16>(tmk, tmv, a, ctas, st);
   if (rows == 32) return launch_attention<kHalf, kDim, 32>(tmk, tmv, a, ctas, st);
-  if constexpr (kDim == 128) {
-    if (rows == 64) return launch_attention<kHalf, kDim, 64>(tmk, tmv, a, ctas, st);
-  }
   if (rows == 128) return launch_attention_wide<kHalf, kDim, 128>(tmk, tmv, a, ctas, st);
   return launch_attention_wide<kHalf, kDim, 256>(tmk, tmv, a, ctas, st);
 }
@@ -257,7 +255,6 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   a.scale_log2 = std::fabs(p->scale) * 1.4426950408889634f;
   a.q_flip = p->scale < 0.f ? 0x80008000u : 0u;
   a.k_combo = static_cast<int>(k_combo), a.v_combo = static_cast<int>(v_combo);
-  a.mask_words = p->mask_words;
   const unsigned int group = static_cast<unsigned int>(p->heads / p->kv_heads);
   a.group_magic = group == 1 ? 0u : static_cast<unsigned int>(((uint64_t(1) << 32) + group - 1) / group);
   uint8_t* base = static_cast<uint8_t*>(p->scratch);

@@ -4,11 +4,15 @@
 //   out = sum_l exp(s_l) V_l / sum_l exp(s_l)   (0 where it sees nothing), times sigmoid(gate) if given.
 //
 // Bound: the cache is read once (4 * dim bytes a token and kv head), so up to a few dozen rows a kv head the kernel
-// is a stream of K and V tiles from HBM; the matrix products only have to keep up.
+// is a stream of K and V tiles from HBM; the matrix products only have to keep up. Measured with the join, 8 kv heads of
+// 128, bf16: 537 MB of cache (one token of 64 heads over 131072 entries) in 84.2 us = 6.38 TB/s, 0.97 of a plain copy's
+// rate; 336 MB (32 requests of 1024 to 4096 entries, pages of 16) in 58.5 us = 5.75 TB/s, 0.88: about 3 us pass before
+// the first tile and 3 us in the join. Short calls are latency: 700 entries of 2 heads of 64 take 9.5 us, of which the
+// cut of the runs is 1 us, the first Q and K 2 us and the join 2.4 us.
 //
 // Shape. The rows of a request that share a kv head (tokens x heads / kv_heads) are one operand, cut into row tiles of
-// kRows (16, 32 or 64; more rows take the rows-as-M kernel of tree_attn_wide.cuh). Tokens are the tensor cores'
-// M: a tile of 128 cached tokens (two at dim 64 and up to 32 rows) gives
+// kRows (16 or 32; more rows take the rows-as-M kernel of tree_attn_wide.cuh). Tokens are the tensor cores'
+// M: a tile of 128 cached tokens (256 at dim 64) gives
 //   S^T [128 tokens x kRows] = K [128 x dim] . Q^T        (UMMA M = 128, N = kRows; K as stored, K-major)
 //   O^T [dim x kRows]       += V^T [dim x 128] . P^T      (UMMA M = 128, N = kRows; V as stored, M-major)
 // so both operands from the cache enter as the TMA wrote them, few rows cost few columns (N = 16) instead of
@@ -60,7 +64,7 @@ struct AttnArgs {
   long long k_page, k_head, k_slot, v_page, v_head, v_slot;
   long long table_row, mask_row;
   long long pages;
-  int requests, tokens, max_draft, table_cols, heads, kv_heads, page, mask_words;
+  int requests, tokens, max_draft, table_cols, heads, kv_heads, page;
   int k_combo, v_combo;      // page stride / head stride: a (page, head) pair is one coordinate of the maps
   unsigned int group_magic;  // row / (heads / kv_heads) = umulhi(row, magic); 0: the group is one head
   float scale_log2;          // |scale| * log2(e)
@@ -86,20 +90,19 @@ __device__ __forceinline__ int attn_token(const AttnArgs& a, int row) {
 template <int kDim, int kRows>
 struct AttnShape {
   static constexpr int kHalves = kDim / 64;
-  static constexpr int kTG = kDim == 64 && kRows <= 32 ? 2 : 1;   // 128-token groups a tile
-  static constexpr int kCG = kRows <= 32 ? 1 : kRows / 32;        // column groups: at most 32 rows of Q a thread
+  static_assert(kRows == 16 || kRows == 32, "rows");
+  static constexpr int kTG = kDim == 64 ? 2 : 1;                  // 128-token groups a tile
   static constexpr int kTok = 128 * kTG;                          // cached tokens a tile
-  static constexpr int kCols = kRows / kCG;
-  static constexpr int kSoft = 128 * kTG * kCG;                   // softmax threads
+  static constexpr int kSoft = 128 * kTG;                         // softmax threads
   static constexpr int kThreads = 64 + kSoft + 32;                // producer, UMMA, softmax, row loader
   static constexpr int kStage = kTok * kDim * 2;                  // one K or V tile
   static constexpr int kQ = kRows * kDim * 2;
   static constexpr int kP = kTok * kRows * 2;
   static constexpr int kNP = 2;                                   // P buffers
-  static constexpr int kNK = kDim == 64 && kRows == 64 ? 5 : 3;
-  static constexpr int kNV = kDim == 64 ? (kRows == 32 ? 2 : kNK) : (kRows <= 32 ? 3 : 2);
+  static constexpr int kNK = 3;
+  static constexpr int kNV = kDim == 64 && kRows == 32 ? 2 : 3;
   static constexpr int kTmemO = 2 * kTG * kRows;                  // after two buffers of S^T
-  static constexpr int kTmem = kTmemO + kRows <= 64 ? 64 : (kTmemO + kRows <= 128 ? 128 : (kTmemO + kRows <= 256 ? 256 : 512));
+  static constexpr int kTmem = kTmemO + kRows <= 64 ? 64 : (kTmemO + kRows <= 128 ? 128 : 256);
   static constexpr int kOffV = kNK * kStage, kOffQ = kOffV + kNV * kStage, kOffP = kOffQ + kQ, kOffSmall = kOffP + kNP * kP;
   // ref, rescale, 1 / sum [kRows]; row ids [2][kRows]; red [4 kTG][kRows]; mask words [2][kRows][9]; segments; barriers.
   static constexpr int kSmall = kRows * 4 * 5 + 4 * kTG * kRows * 4 + kRows * 72 + 128 + (2 * kNK + 2 * kNV + 13) * 8 + 64;
@@ -524,7 +527,7 @@ template <bool kHalf, int kDim, int kRows>
 __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     tree_attn_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, const AttnArgs a) {
   using Sh = AttnShape<kDim, kRows>;
-  constexpr int kHalves = Sh::kHalves, kNK = Sh::kNK, kNV = Sh::kNV, kNP = Sh::kNP, kCols = Sh::kCols, kTok = Sh::kTok;
+  constexpr int kHalves = Sh::kHalves, kNK = Sh::kNK, kNV = Sh::kNV, kNP = Sh::kNP, kTok = Sh::kTok;
   constexpr int kTG = Sh::kTG, kSoft = Sh::kSoft;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_align<1024>(smem_raw);
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       constexpr uint32_t kType = kHalf ? 0u : ((1u << 7) | (1u << 10));
       constexpr uint32_t kShape = (1u << 4) | (static_cast<uint32_t>(kRows >> 3) << 17) | (8u << 24);
       constexpr uint32_t idesc_s = kShape | kType, idesc_o = kShape | kType | (1u << 15) | (1u << 16);
-      constexpr int kPRow = kRows >= 64 ? 128 : kRows * 2;  // bytes of a token's row of P
+      constexpr int kPRow = kRows * 2;  // bytes of a token's row of P
       constexpr uint64_t k_bits = attn_desc_bits(128, 1024 * kHalves, 16);
       constexpr uint64_t v_bits = attn_desc_bits(128, 1024 * kHalves, kHalves > 1 ? 1024 : 0);
       constexpr uint64_t p_bits = attn_desc_bits(kPRow, 8 * kPRow, 0);
@@ -650,14 +653,10 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
     if (plan.work)
       attn_load_rows<kTok, kRows, kRows, 16, kDim, 32>(a, plan, lane, q_s, segs, all_words, row_ids, q_full, q_empty, seg_done);
   } else {
-    // ---- softmax: thread = one token of the tile (a TMEM lane of its token group), its group's columns ----
+    // ---- softmax: thread = one token of the tile (a TMEM lane of its token group), all rows ----
     const int tid = static_cast<int>(threadIdx.x) - 64;
-    const int tg = (tid >> 7) % kTG, cg = (tid >> 7) / kTG;
+    const int tg = tid >> 7;
     const int quarter = warp & 3, tl = quarter * 32 + lane, token = tg * 128 + tl;
-    const int c0 = cg * kCols;
-    const int bar = 1 + cg;
-    constexpr int kGroup = 128 * kTG;  // threads that share columns
-    const int gtid = tid % kGroup;
     const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
     const float kNegInf = __int_as_float(0xff800000);
     const float c = a.scale_log2;
@@ -666,7 +665,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
       uint32_t n = 0;  // tiles done in this run
       uint32_t v_slot = 0, v_phase = 0;
       bool ok = true;
-      float l[kCols];
+      float l[kRows];
       for (int k = 0;; ++k) {
         // ---- the segment's rows --------------------------------------------------------------------
         ok = mbar_wait_idle(&q_full[k & 1], (k >> 1) & 1, kErrAttnSoftmax);
@@ -674,8 +673,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         const AttnSeg s = segs[k & 1];
         if (s.i1 <= s.i0) break;
         const int rows = min(kRows, s.r.rows - s.row0);
-        const int full = min(kRows, (rows + 15) & ~15);  // columns that are computed
-        const int live = min(max(full - c0, 0), kCols);  // of this group
+        const int live = min(kRows, (rows + 15) & ~15);  // columns that are computed
         const uint32_t* words = all_words + (k & 1) * kRows * 9;
         const int* row_id = row_ids + (k & 1) * kRows;
         int* odd_v = odd_vs + (k & 1);
@@ -683,7 +681,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         if (tid == 0) odd_vs[(k + 1) & 1] = 0;
         bar_named(8, kSoft);
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) l[j] = 0.f;
+        for (int j = 0; j < kRows; ++j) l[j] = 0.f;
         const bool lone = s.r.drafted == 1 && !a.mask;  // one token, which sees itself
 
         // ---- tiles ---------------------------------------------------------------------------------
@@ -693,13 +691,13 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           // P's buffer is free, and with two of them PV of two tiles ago is done, once this has passed.
           if (n >= static_cast<uint32_t>(kNP)) ok = mbar_wait_idle(&pv_done[(n - kNP) & 1u], ((n - kNP) >> 1) & 1u, kErrAttnSoftmax) && ok;
           tc_fence_after();
-          float x[kCols];
-          const uint32_t ts = tmem + ((n & 1u) * kTG + tg) * kRows + c0 + lanes;
+          float x[kRows];
+          const uint32_t ts = tmem + ((n & 1u) * kTG + tg) * kRows + lanes;
 #pragma unroll
-          for (int cc = 0; cc < kCols; cc += 16)
+          for (int cc = 0; cc < kRows; cc += 16)
             if (cc < live) attn_ld16(ts + cc, x + cc);
 #pragma unroll
-          for (int cc = 0; cc < kCols; cc += 16)
+          for (int cc = 0; cc < kRows; cc += 16)
             if (cc < live) attn_ld_wait(x + cc);
           const int pos = i * kTok + token;
           const bool edge = (i + 1) * kTok > s.r.ctx;  // the tile reaches past the context
@@ -711,17 +709,17 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
             if (!lone && seen && j >= 0) {
               seen = 0u;
 #pragma unroll
-              for (int k = 0; k < kCols; ++k)
-                if (k < live) seen |= ((words[(c0 + k) * 9 + (j >> 5)] >> (j & 31)) & 1u) << k;
+              for (int k = 0; k < kRows; ++k)
+                if (k < live) seen |= ((words[k * 9 + (j >> 5)] >> (j & 31)) & 1u) << k;
             }
 #pragma unroll
-            for (int k = 0; k < kCols; ++k) x[k] = (seen >> k) & 1u ? x[k] * c : kNegInf;
+            for (int k = 0; k < kRows; ++k) x[k] = (seen >> k) & 1u ? x[k] * c : kNegInf;
           }
           float over[4] = {kNegInf, kNegInf, kNegInf, kNegInf};  // how far a score passes its reference
 #pragma unroll
-          for (int cc = 0; cc < kCols; cc += 4) {
+          for (int cc = 0; cc < kRows; cc += 4) {
             if (cc < live) {
-              const float4 m = *reinterpret_cast<const float4*>(ref + c0 + cc);
+              const float4 m = *reinterpret_cast<const float4*>(ref + cc);
               over[0] = fmaxf(over[0], fmaf(x[cc], cm, -m.x));
               over[1] = fmaxf(over[1], fmaf(x[cc + 1], cm, -m.y));
               over[2] = fmaxf(over[2], fmaf(x[cc + 2], cm, -m.z));
@@ -729,23 +727,23 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
             }
           }
           const bool past = fmaxf(fmaxf(over[0], over[1]), fmaxf(over[2], over[3])) > kAttnSlack;
-          if (bar_any(bar, kGroup, past || !ok)) {
-            if (bar_any(bar, kGroup, !ok)) {
+          if (bar_any(8, kSoft, past || !ok)) {
+            if (bar_any(8, kSoft, !ok)) {
               ok = false;
               break;
             }
             // Move the references to the true maxima and rescale what was summed against the old ones.
 #pragma unroll
-            for (int cc = 0; cc < kCols; cc += 16) {
+            for (int cc = 0; cc < kRows; cc += 16) {
               float top[16];
 #pragma unroll
               for (int j = 0; j < 16; ++j) top[j] = cc < live ? x[cc + j] * cm : kNegInf;
               warp_fold16<true>(top, lane);
-              if (!(lane & 1)) red[(tg * 4 + quarter) * kRows + c0 + cc + (lane >> 1)] = top[0];
+              if (!(lane & 1)) red[(tg * 4 + quarter) * kRows + cc + (lane >> 1)] = top[0];
             }
-            bar_named(bar, kGroup);
-            if (gtid < kCols) {
-              const int col = c0 + gtid;
+            bar_named(8, kSoft);
+            if (tid < kRows) {
+              const int col = tid;
               const float old = ref[col];
               float now = old;
 #pragma unroll
@@ -753,22 +751,22 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
               ref[col] = now;
               rescale[col] = ex2(old - now);
             }
-            bar_named(bar, kGroup);
+            bar_named(8, kSoft);
             if (i > s.i0) {
 #pragma unroll
-              for (int j = 0; j < kCols; ++j)
-                if (j < live) l[j] *= rescale[c0 + j];
+              for (int j = 0; j < kRows; ++j)
+                if (j < live) l[j] *= rescale[j];
               ok = mbar_wait_idle(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax) && ok;
               tc_fence_after();
 #pragma unroll
-              for (int cc = 0; cc < kCols; cc += 16) {
+              for (int cc = 0; cc < kRows; cc += 16) {
                 if (cc < live && ((cc >> 4) & (kTG - 1)) == tg) {
                   float o[16];
-                  attn_ld16(tmem_o + c0 + cc + lanes, o);
+                  attn_ld16(tmem_o + cc + lanes, o);
                   attn_ld_wait(o);
 #pragma unroll
-                  for (int k = 0; k < 16; ++k) o[k] *= rescale[c0 + cc + k];
-                  attn_st16(tmem_o + c0 + cc + lanes, o);
+                  for (int k = 0; k < 16; ++k) o[k] *= rescale[cc + k];
+                  attn_st16(tmem_o + cc + lanes, o);
                 }
               }
               attn_st_wait();
@@ -777,9 +775,9 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           // P, rounded, as the second product reads it (a score that is not seen is -inf, its P zero).
           const uint32_t pt = smem_u32(p_s + (n % kNP) * Sh::kP);
 #pragma unroll
-          for (int cc = 0; cc < kCols; cc += 8) {
+          for (int cc = 0; cc < kRows; cc += 8) {
             if (cc < live) {
-              const float4 m0 = *reinterpret_cast<const float4*>(ref + c0 + cc), m1 = *reinterpret_cast<const float4*>(ref + c0 + cc + 4);
+              const float4 m0 = *reinterpret_cast<const float4*>(ref + cc), m1 = *reinterpret_cast<const float4*>(ref + cc + 4);
               const float m[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
               uint32_t w[4];
 #pragma unroll
@@ -787,21 +785,18 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
                 w[k] = pack16x2<kHalf>(ex2(fmaf(x[cc + 2 * k], cm, -m[2 * k])), ex2(fmaf(x[cc + 2 * k + 1], cm, -m[2 * k + 1])));
                 add16x2<kHalf>(w[k], l[cc + 2 * k], l[cc + 2 * k + 1]);
               }
-              const int ch = (c0 + cc) >> 3;
+              const int ch = cc >> 3;
               uint32_t at;
               if constexpr (kRows == 16) at = token * 32 + ((ch ^ ((token >> 2) & 1)) << 4);
-              else if constexpr (kRows == 32) at = token * 64 + ((ch ^ ((token >> 1) & 3)) << 4);
-              else at = token * 128 + ((ch ^ (token & 7)) << 4);
+              else at = token * 64 + ((ch ^ ((token >> 1) & 3)) << 4);
               st_shared_v4u(pt + at, w[0], w[1], w[2], w[3]);
             }
           }
-          if (cg == 0) {
-            // In the last tile or two of a request.
-            const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && s.r.drafted > 1;
-            if (ragged || drafted) {
-              ok = mbar_wait_idle(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
-              attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), token, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);
-            }
+          // In the last tile or two of a request.
+          const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && s.r.drafted > 1;
+          if (ragged || drafted) {
+            ok = mbar_wait_idle(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
+            attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), token, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);
           }
           if (++v_slot == kNV) v_slot = 0, v_phase ^= 1u;
           fence_proxy_async_shared();
@@ -812,9 +807,9 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         // ---- end of the segment: finish the row tile, or leave a partial ---------------------------
         const bool whole = s.i0 == 0 && s.i1 == s.r.tiles;
 #pragma unroll
-        for (int cc = 0; cc < kCols; cc += 16) {
+        for (int cc = 0; cc < kRows; cc += 16) {
           warp_fold16<false>(l + cc, lane);
-          if (!(lane & 1)) red[(tg * 4 + quarter) * kRows + c0 + cc + (lane >> 1)] = l[cc];
+          if (!(lane & 1)) red[(tg * 4 + quarter) * kRows + cc + (lane >> 1)] = l[cc];
         }
         if (ok) ok = mbar_wait_idle(&pv_done[(n - 1) & 1u], ((n - 1) >> 1) & 1u, kErrAttnSoftmax);
         ok = !bar_any(8, kSoft, !ok);
@@ -822,8 +817,8 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
         tc_fence_after();
         // The run that starts inside a row tile keeps its partial first, the one that ends inside it second.
         const int slot = (blockIdx.x * 2 + (s.i0 > 0 ? 0 : 1)) * kRows;
-        if (gtid < kCols) {
-          const int col = c0 + gtid;
+        if (tid < kRows) {
+          const int col = tid;
           float sum = 0.f;
 #pragma unroll
           for (int w = 0; w < 4 * kTG; ++w) sum += red[w * kRows + col];
@@ -834,19 +829,19 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
           cross.first = s.r.first, cross.row0 = s.row0, cross.rows = rows, cross.head = s.head;
           cross.last = plan.runs.of(s.unit0 + s.r.tiles - 1);
         }
-        bar_named(bar, kGroup);
+        bar_named(8, kSoft);
         const int odd = *odd_v;
 #pragma unroll
-        for (int cc = 0; cc < kCols; cc += 16) {
+        for (int cc = 0; cc < kRows; cc += 16) {
           if (cc < live && ((cc >> 4) & (kTG - 1)) == tg) {
             float o[16];
-            attn_ld16(tmem_o + c0 + cc + lanes, o);
+            attn_ld16(tmem_o + cc + lanes, o);
             uint16_t gv[16];
             const bool mine_o = tl < kDim;
             if (whole && a.gate && mine_o) {
 #pragma unroll
               for (int k = 0; k < 16; ++k) {
-                const int id = row_id[c0 + cc + k];
+                const int id = row_id[cc + k];
                 gv[k] = __ldg(a.gate + (s.r.first + (id >> 16)) * a.gate_token + (id & 0xFFFF) * a.gate_head + tl);
               }
             }
@@ -863,13 +858,13 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
                   if (!(fabsf(v) < __int_as_float(0x7f800000)))
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
-                      if ((words[(c0 + cc + k) * 9 + (j >> 5)] >> (j & 31)) & 1u) o[k] += v;
+                      if ((words[(cc + k) * 9 + (j >> 5)] >> (j & 31)) & 1u) o[k] += v;
                 }
               }
               if (whole) {
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                  const int col = c0 + cc + k, id = row_id[col];
+                  const int col = cc + k, id = row_id[col];
                   float v = o[k] * inv[col];
                   if (a.gate) v = __fdividef(v, 1.f + __expf(-lo16<kHalf>(gv[k])));
                   if (col < rows)
@@ -879,7 +874,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
               } else {
 #pragma unroll
                 for (int k = 0; k < 16; ++k)
-                  if (c0 + cc + k < rows) a.part_o[static_cast<long long>(slot + c0 + cc + k) * kDim + tl] = o[k];
+                  if (cc + k < rows) a.part_o[static_cast<long long>(slot + cc + k) * kDim + tl] = o[k];
               }
             }
           }
@@ -902,7 +897,9 @@ __host__ __device__ constexpr int attn_join_rows(int rows) { return rows >= 128 
 // Joins the partials of the row tiles that cross runs: grid (runs, parts of the rows), 8 warps, of which each
 // row has 8 (16 rows) to 1 (128 and more) that take the runs in turn, four partials on their way at once. A
 // partial weighs 2^(its reference - the largest); the order of the sums is fixed. Latency is its cost: one load of
-// what crosses here, then everything else together.
+// what crosses here, then everything else together (2.4 us after one token over 700 entries, 4 us with 52 rows; 14 us
+// for the 38 MB of partials of 256-row tiles). A CTA takes few rows: with four rows a warp 8 requests x 16 tokens took
+// 21 us in all, 17 so.
 template <bool kHalf, int kDim, int kRows>
 __global__ void __launch_bounds__(256) tree_attn_join_kernel(const AttnArgs a) {
   constexpr int kN = kDim / 32, kBlock = attn_join_rows(kRows), kPerRow = 8 / kBlock;

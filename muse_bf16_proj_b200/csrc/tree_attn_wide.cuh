@@ -1,4 +1,4 @@
-// tree_attention with many rows a kv head (more than 64): rows as the tensor cores' M.
+// tree_attention with many rows a kv head (more than 32): rows as the tensor cores' M.
 //
 // A unit is up to 256 rows (tokens x heads of a group) of one request and kv head: one or two row tiles of 128, which
 // share every K and V tile that is brought in. For a row tile and 128 cached tokens
@@ -6,7 +6,12 @@
 //   O [128 rows x dim]       += P . V              (P from tensor memory over S's columns, V as stored, N-major)
 // A row is a TMEM lane and one softmax thread's, so its maximum, its references and its sums need no other thread,
 // and P never passes through shared memory. Bound: at 2 x 128 rows the two products take 1024 tensor cycles a tile at
-// dim 128 and its 16384 exponentials as many cycles of the exponential unit; K and V come in once for both.
+// dim 128 and its 16384 exponentials as many cycles of the exponential unit; K and V come in once for both. Measured: 16
+// requests of 64 tokens, 64 heads over 8 of 128, up to 8192 entries (174 GFLOP) in 205 us with the join = 850 TFLOP/s,
+// 0.51 of a dense product's rate, the tensor cores busy 44 % of the cycles and no other unit above that: one S at a time
+// passes from the products to a softmax and back, and each of those hand-offs is on the chain (TMEM has no room for a
+// second S at dim 128). 33 to 128 rows over 822 MB of cache take 132 to 141 us = 6.2 to 5.8 TB/s; 52 rows over 84 MB
+// (11 requests of up to 13 tokens) take 25 us against 12.7 of bytes: the start, the row tiles' ends and the join.
 //
 // Two row tiles alternate ("pair"): while one's softmax runs, the tensor cores do the other's products. Each has its
 // own warpgroup and O. One row tile ("lone"): each warpgroup takes 64 of a tile's 128 tokens of every row; the two
