@@ -28,8 +28,9 @@ extern "C" {
 #define MUSE_ERR_SHAPE (-3)     /* shape outside what the chosen kernel supports */
 #define MUSE_ERR_CAPACITY (-4)  /* a caller-provided buffer is too small (see the count written) */
 #define MUSE_ERR_CUDA (-5)      /* a CUDA runtime / driver call failed (message has the name) */
-#define MUSE_ERR_TIMEOUT (-6)   /* the device error word was set: a kernel's bounded wait expired, or the
-                                 * device encoder skipped an escape outside its buffer (0x501) */
+#define MUSE_ERR_TIMEOUT (-6)   /* the device error word was set: a kernel's bounded wait expired, the
+                                 * device encoder skipped an escape outside its buffer (0x501), or a kernel
+                                 * found an index out of range in device data (0xA01 .. 0xB03) */
 #define MUSE_ERR_PLAN (-7)      /* unknown kernel id or plan field out of range */
 
 /* Kernels a plan can name. */
@@ -142,7 +143,9 @@ int muse_sm_count(int* out);
 
 /*
  * Reads the device error word that bounded waits set on timeout (and the device encoder on an
- * escape outside its buffer, 0x501), writes it to *code (0 = none) and clears it. Synchronizes `stream`. Returns MUSE_ERR_TIMEOUT when it was set.
+ * escape outside its buffer, 0x501; muse_rope_append and muse_tree_attention on an index out of
+ * range, 0xA01, 0xA02 and 0xB01 .. 0xB03), writes it to *code (0 = none) and clears it.
+ * Synchronizes `stream`. Returns MUSE_ERR_TIMEOUT when it was set.
  * No counterpart in the reference (its kernels have no bounded waits).
  */
 int muse_device_error(int* code, void* stream);

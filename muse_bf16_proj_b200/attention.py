@@ -10,7 +10,8 @@ projections runs::
     a = tree_attention(q, k_pages, v_pages, page_table, context, starts, max_draft, tree_mask, gate=gate)
     y = project(a.view(M, Hq * D), state, "o")
 
-The cache is two tensors [pages, kv_heads, page_size, dim] (any page, head and entry strides). Request b
+The cache is two tensors [pages, kv_heads, page_size, dim] (any order of pages, heads
+and entries in memory whose page stride is a multiple of the head stride). Request b
 keeps its tokens in the pages of row b of ``page_table``; a token's *slot* is page * page_size + entry
 (``page_slots``). Calls launch on torch's current stream, allocate with torch's caching allocator only,
 do not synchronise and can be captured in a CUDA graph. A position, slot, page or request size out of
