@@ -443,8 +443,7 @@ int muse_decode12(const uint8_t* planes, const uint8_t* bases, const int32_t* es
  * operators a decode, verify or prompt step runs between its qkv_gate and o projections (16 query heads and
  * 2 key/value heads of 64 plus a 16 x 64 gate on each GPU) and after its router. Strides are in elements, the
  * last dimension of every tensor is contiguous. All pointers are device pointers; launches use programmatic
- * dependent launch and read no input before the previous grid in the stream has completed, but for constants
- * named at each.
+ * dependent launch and read no input before the previous grid in the stream has completed.
  */
 
 /* 16-bit types of q, k, v, the cache, the gate and the output. */
@@ -530,7 +529,7 @@ int muse_tree_attention_scratch_bytes(const MuseTreeAttention* args, int64_t* by
  * g * experts / groups .. are group g, worth its best choice (with a bias: its best two added); only the best
  * top_groups groups stay. Chosen in descending order, ties to the lowest index. weights = the chosen scores, divided
  * by their sum if renormalize (0 where that is 0), times scale. A NaN logit counts as -inf; an expert of -inf is
- * chosen after every other and weighs 0. `bias` is a constant: it may be read before the previous grid ends.
+ * chosen after every other and weighs 0.
  */
 typedef struct MuseRoute {
   const void* logits;       /* [tokens, experts] */

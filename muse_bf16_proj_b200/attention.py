@@ -242,7 +242,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         so = (heads * dim, dim)
     if scale is None:
         scale = dim ** -0.5
-    need = _scratch_bytes(dev, requests, max_draft, heads, kv_heads, dim)
+    need = _scratch_bytes(dev, max_draft, heads, kv_heads, dim)
     scratch = torch.empty(need, dtype=torch.uint8, device=q.device)
     _call(dev, _lib.tree_attention, _lib.PACK_TREE_ATTENTION(
         q.data_ptr(), gates, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table, lengths, first, mask, scratch.data_ptr(), need,
@@ -252,8 +252,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
 
 
 @functools.lru_cache(maxsize=None)
-def _scratch_bytes(dev: int, requests: int, max_draft: int, heads: int, kv_heads: int, dim: int) -> int:
+def _scratch_bytes(dev: int, max_draft: int, heads: int, kv_heads: int, dim: int) -> int:
     """What the split of the cache needs, by the sizes that decide it."""
     with torch.cuda.device(dev):
-        return _lib.tree_attention_scratch_bytes(_lib.MuseTreeAttention(requests=requests, max_draft=max_draft, heads=heads, kv_heads=kv_heads,
-                                                                        dim=dim, scale=1.0))
+        return _lib.tree_attention_scratch_bytes(_lib.MuseTreeAttention(max_draft=max_draft, heads=heads, kv_heads=kv_heads, dim=dim, scale=1.0))

@@ -79,7 +79,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
   __shared__ float choices[kRouteWarps][kJ * 128];  // group scan only
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const float kNegInf = __int_as_float(0xff800000);
-  // The bias is a constant of the model: loaded before the wait for the previous grid.
+  pdl_wait();
+  pdl_launch_dependents();
+  const int token = blockIdx.x * kRouteWarps + warp;
+  if (token >= a.tokens) return;
+  const long long base = token * a.row;
   float bias[kN];
 #pragma unroll
   for (int j = 0; j < kJ; ++j) {
@@ -92,11 +96,6 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
       for (int i = 0; i < 4; ++i) bias[j * 4 + i] = a.bias && e + i < a.count ? __ldg(a.bias + e + i) : 0.f;
     }
   }
-  pdl_wait();
-  pdl_launch_dependents();
-  const int token = blockIdx.x * kRouteWarps + warp;
-  if (token >= a.tokens) return;
-  const long long base = token * a.row;
 
   float x[kN];
 #pragma unroll

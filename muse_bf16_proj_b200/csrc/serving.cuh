@@ -204,7 +204,7 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   if (p->pages < 1 || p->table_cols < 1) return fail(MUSE_ERR_INVALID, "tree_attention: pages and table_cols must be positive");
   if (static_cast<int64_t>(p->table_cols) * p->page_size > (int64_t(1) << 30) || p->pages > (int64_t(1) << 31) - 1)
     return fail(MUSE_ERR_SHAPE, "tree_attention: a request's pages must hold at most 2^30 entries, the cache fewer than 2^31 pages");
-  const int64_t tiles = static_cast<int64_t>(p->table_cols) * p->page_size / 128 + 1;
+  const int64_t tiles = static_cast<int64_t>(p->table_cols) * p->page_size / 128 + 1 + muse::kAttnEnds;
   const int64_t units = static_cast<int64_t>(p->kv_heads) * (static_cast<int64_t>(p->max_draft) * (p->heads / p->kv_heads) / 128 + 1);
   if (p->requests > 0 && tiles * units > ((int64_t(1) << 31) - 1) / p->requests)
     return fail(MUSE_ERR_SHAPE, "tree_attention: requests x page table x kv_heads x max_draft is too large (more than 2^31 tiles)");

@@ -134,3 +134,20 @@ def test_same_bits_as_elementary_operations():
 def test_no_tokens():
     w, e = route(torch.zeros((0, 64), device="cuda"), 4)
     assert w.shape == e.shape == (0, 4)
+
+
+def test_bias_written_just_before():
+    """A balance bias that the previous launch wrote counts, another every time."""
+    logits = grid_logits(64, 256, 5)
+    offsets = (torch.arange(256, device="cuda") % 7 - 3).float() / 4
+    bias = torch.zeros(256, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    route(logits, 8, scoring="sigmoid", bias=bias, groups=8, top_groups=4)
+    with torch.cuda.graph(graph):
+        bias.copy_(offsets)
+        _, e = route(logits, 8, scoring="sigmoid", bias=bias, groups=8, top_groups=4)
+        offsets.copy_(offsets.roll(1))
+    for _ in range(5):
+        want = route64(logits, 8, "sigmoid", offsets.clone(), 8, 4, True, 1.0)[1]
+        graph.replay()
+        assert torch.equal(e.cpu(), want)
