@@ -8,7 +8,7 @@
 // one coalesced 16-byte (8-byte) load a lane for each 128 experts. A choice becomes an unsigned key in its
 // order, and a lane keeps its best two with their places; each of the k rounds is one warp-wide maximum of the
 // lanes' best keys and one warp-wide minimum of the index among its holders, after which the holder's second moves
-// up (17.0 us for 8192 tokens of 256 experts where the holder searched its eight again, 13.9 so). Lane r then
+// up (17.0 us for 8192 tokens of 256 experts where the holder searched its eight again, 14 so). Lane r then
 // computes the r-th expert's weight from its logit, so the k weights cost one pass. Bound: latency of that chain
 // (5 us for one token at k = 8, 3 us of them the launch) until enough tokens are there to fill the SMs' warps, then
 // the issue of its instructions (66 % of all slots at 8192 tokens); the bytes (4 a logit, 8.9 MB and 1.4 us there)
