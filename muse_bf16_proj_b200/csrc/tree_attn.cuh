@@ -39,7 +39,8 @@
 //
 // Entries that no row may see: tokens past the request's end are not loaded (or are whatever the page holds)
 // and their V rows are zeroed in shared memory, because 0 x NaN is NaN; drafted tokens, which some rows see and
-// others not, have non-finite V entries replaced by zero and added back at the end to the rows that do see them.
+// others not (a mask may hide a request's only one from all of them), have non-finite V entries replaced by zero and
+// added back at the end to the rows that do see them.
 #pragma once
 
 #include "ptx.cuh"
@@ -792,8 +793,8 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
               st_shared_v4u(pt + at, w[0], w[1], w[2], w[3]);
             }
           }
-          // In the last tile or two of a request.
-          const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && s.r.drafted > 1;
+          // In the last tile or two of a request. A lone token sees itself: only then is no drafted entry hidden from a row.
+          const bool ragged = (i + 1) * kTok > s.r.kv, drafted = edge && !lone;
           if (ragged || drafted) {
             ok = mbar_wait_idle(&v_full[v_slot], v_phase, kErrAttnSoftmax) && ok;
             attn_clean_v<kHalf, kDim>(smem_u32(ring_v + v_slot * Sh::kStage), token, pos >= s.r.kv, drafted && pos >= s.r.ctx, odd_v);

@@ -352,7 +352,8 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
           const int i = s.i0 + (kPair ? v >> 1 : v), col0 = kPair ? 0 : wg * 64;
           const bool edge = (i + 1) * kTok > s.r.ctx;  // the tile reaches past the context
           if (wg == 0 && edge) {
-            const bool ragged = (i + 1) * kTok > s.r.kv, drafted = s.r.drafted > 1;
+            // One token without a mask sees itself: only then is no drafted entry hidden from a row.
+            const bool ragged = (i + 1) * kTok > s.r.kv, drafted = s.r.drafted > 1 || a.mask;
             if (ragged || drafted) {
               // The place's fill before is complete once PV of two products ago is: only then does the parity name this fill.
               if (v >= 2) ok = mbar_wait_idle(&pv_done[buffer], ((n - 2) >> 1) & 1u, kErrAttnSoftmax) && ok;

@@ -292,3 +292,18 @@ def test_tree_mask_words():
     got = tree_mask(parents, starts, 37)
     assert got.shape == (40, 2) and got[:3, 0].tolist() == [1, 3, 5]
     assert got[3 + 31].tolist() == [-1, 0] and got[39].tolist() == [-1, 31]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("drafts,hq", [([1, 1, 1], 8), ([1, 6, 1], 8), ([1, 12, 1], 8), ([1, 40, 1], 16)])
+@pytest.mark.parametrize("poison", [float("nan"), float("inf"), -float("inf")])
+def test_a_hidden_token_of_one_does_not_matter(drafts, hq, d, poison):
+    """A request's only drafted token with an empty mask row: its own entry may hold anything, and over no context
+    its row is zero. Row counts of every variant, contexts of 0, inside a tile, and over many runs."""
+    a = make([0, 30, 3001], drafts, hq, 2, d, 16, torch.bfloat16, gate=True)
+    for b, context in ((0, 0), (2, 3001)):
+        a["tree_mask"][int(a["starts"][b])] = 0
+        page = a["page_table"][b, context // 16].long()
+        a["k_pages"][page, :, context % 16], a["v_pages"][page, :, context % 16] = poison, poison
+    got = check(a)
+    assert int(torch.count_nonzero(got[0])) == 0
