@@ -144,7 +144,8 @@ int muse_sm_count(int* out);
 /*
  * Reads the device error word that bounded waits set on timeout (and the device encoder on an
  * escape outside its buffer, 0x501; muse_rope_append and muse_tree_attention on an index out of
- * range, 0xA01, 0xA02 and 0xB01 .. 0xB03), writes it to *code (0 = none) and clears it.
+ * range, 0xA01, 0xA02 and 0xB01 .. 0xB03), writes it to *code (0 = none) and clears it. The first
+ * code stays until it is read, but for one: the code of a wait takes the place of an index code.
  * Synchronizes `stream`. Returns MUSE_ERR_TIMEOUT when it was set.
  * No counterpart in the reference (its kernels have no bounded waits).
  */

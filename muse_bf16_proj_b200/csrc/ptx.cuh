@@ -40,12 +40,24 @@ __device__ __forceinline__ unsigned long long globaltimer() {
   return t;
 }
 
-__device__ __forceinline__ void report_error(unsigned int code) { atomicCAS(&g_dev_error, 0u, code); }
-
 // An argument out of its range (0xA01 .. 0xA0F, 0xB01 .. 0xB0F) concerns one token or request; nothing else stops for it.
+__device__ __forceinline__ bool index_code(unsigned int code) { return code >= 0xA00u && (code & 0xF0u) == 0u; }
+
+// Records `code` in the device error word. The first code stays, but the code of a wait that gave up takes the place of
+// an index code: error_raised() goes by the word, and what stops for a wait must not miss it. A failed exchange is tried
+// again from what it found (another thread's index code, or 0 where the host has just cleared the word).
+__device__ __forceinline__ void report_error(unsigned int code) {
+  unsigned int from = 0u;
+  for (int i = 0; i < 4; ++i) {
+    const unsigned int now = atomicCAS(&g_dev_error, from, code);
+    if (now == from || (now != 0u && (index_code(code) || !index_code(now)))) return;
+    from = now;
+  }
+}
+
 __device__ __forceinline__ bool error_raised() {
   const unsigned int code = *reinterpret_cast<volatile unsigned int*>(&g_dev_error);
-  return code != 0u && !(code >= 0xA00u && (code & 0xF0u) == 0u);
+  return code != 0u && !index_code(code);
 }
 
 // ---- per-CTA timestamp trace (off unless the host set a buffer) -----------------------------

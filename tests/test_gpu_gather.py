@@ -145,6 +145,39 @@ def test_late_peer_after_a_timeout_ends_with_an_error():
     assert _lib.device_error(stream) == 0
 
 
+def test_a_pending_index_error_does_not_hide_a_timeout():
+    """As above with a bad slot recorded (0xA02) and not read before each rank's call: the waits that give up still replace
+    it in the error word, and rank 0 still publishes no done flag."""
+    from muse_bf16_proj_b200.attention import rope_append, rope_table
+
+    stream = torch.cuda.current_stream().cuda_stream
+    m, n, k = 4, 1024, 2048
+    g = torch.Generator().manual_seed(7)
+    w = (torch.randn((n, k), generator=g) * 0.02).to(torch.bfloat16).cuda()
+    x = torch.randn((m, k), generator=g).to(torch.bfloat16).cuda()
+    tiles = _packed(w, stream)
+    plan = _tile_plan(16, 1)
+    y = [torch.zeros((m, 2 * n), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    ctl = torch.zeros((2, _lib.peer_ctl_bytes()), dtype=torch.uint8, device="cuda")
+    row = torch.zeros((1, 1, 64), dtype=torch.bfloat16, device="cuda")
+    pages = torch.zeros((2, 1, 16, 64), dtype=torch.bfloat16, device="cuda")
+    table = rope_table(64, 4)
+    zero, bad = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.full((1,), 32, dtype=torch.int64, device="cuda")
+    _lib.device_error(stream)  # start from a clear error word
+    for rank, expect in ((0, "0x401"), (1, "0x402")):
+        gat = _lib.MuseGather()
+        gat.world, gat.rank, gat.ldy, gat.col0 = 2, rank, 2 * n, rank * n
+        gat.y[0], gat.y[1] = y[0].data_ptr(), y[1].data_ptr()
+        gat.ctl[0], gat.ctl[1] = ctl[0].data_ptr(), ctl[1].data_ptr()
+        rope_append(row, row, row, zero, bad, pages, pages.clone(), table)
+        _lib.proj_bf16_tiles_gather(x.data_ptr(), tiles.data_ptr(), m, n, k, gat, plan, stream)
+        rope_append(row, row, row, zero, bad, pages, pages.clone(), table)  # nor does a later one take its place
+        with pytest.raises(_lib.MuseError) as err:
+            _lib.device_error(stream)
+        assert expect in str(err.value), (rank, str(err.value))
+    assert _lib.device_error(stream) == 0
+
+
 def _free_port() -> int:
     with socket.socket() as s:
         s.bind(("127.0.0.1", 0))
