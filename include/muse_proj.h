@@ -484,7 +484,9 @@ int muse_rope_append(const MuseRopeAppend* args, void* stream);
 /*
  * Attention of each request's drafted tokens over its cached tokens and the drafted ones before them (a tree, a
  * chain, or a single decoded token). Request b has tokens starts[b] .. starts[b + 1] - 1 (none is allowed), whose
- * keys and values are already in the cache at entries context[b] + j. Every row sees the context; drafted token
+ * keys and values are already in the cache at entries context[b] + j. Tokens before starts[0] and from starts[requests] on
+ * belong to no request (a fixed-size step's padding): their rows of out are 0 (with requests = 0 nothing is launched and
+ * out stays as it is). Every row sees the context; drafted token
  * j where bit j % 32 of word j / 32 of its mask row is set (mask NULL: its own and every earlier one).
  * out = softmax(scale * q . K) V over what the row sees, 0 where it sees nothing, times sigmoid(gate) if gate is
  * given; FP32 softmax statistics and sums, rounded once (the weights of V to the 16-bit type on the way). Entries of the cache that a row does not see, and what the
@@ -504,7 +506,7 @@ typedef struct MuseTreeAttention {
   const void* v_pages;
   const int32_t* table;     /* [requests, table_cols] page of each page_size entries */
   const int32_t* context;   /* [requests] */
-  const int32_t* starts;    /* [requests + 1], starts[0] = 0, starts[requests] = tokens */
+  const int32_t* starts;    /* [requests + 1], 0 <= starts[0] <= .. <= starts[requests] <= tokens */
   const uint32_t* mask;     /* [tokens, mask_words] or NULL */
   void* scratch;
   int64_t scratch_bytes;

@@ -208,8 +208,9 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of every request's drafted tokens over its cache: out [M, Hq, D].
 
-    Request b has the tokens starts[b] .. starts[b + 1] - 1 of q [M, Hq, D] (``starts`` int32 [B + 1], from 0
-    to M; a request may have none), at most ``max_draft`` (1 .. 256). Its sequence is ``context[b]`` (int32
+    Request b has the tokens starts[b] .. starts[b + 1] - 1 of q [M, Hq, D] (``starts`` int32 [B + 1], rising;
+    a request may have none), at most ``max_draft`` (1 .. 256). Rows before starts[0] and from starts[B] on belong
+    to no request (a fixed-size step's padding) and are 0. Its sequence is ``context[b]`` (int32
     [B]) cached tokens followed by the drafted ones, already appended, in the pages ``page_table[b]`` (int32
     [B, pages of a request]) of the cache [pages, Hkv, page_size, D] (page_size a power of two, 8 .. 1024).
     Each token sees the context and the drafted tokens whose bits its row of ``tree_mask`` (int32 [M, words],
@@ -248,6 +249,8 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         q.data_ptr(), gates, out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), table, lengths, first, mask, scratch.data_ptr(), need,
         sq[0], sq[1], sg[0], sg[1], so[0], so[1], ck[0], ck[1], ck[2], cv[0], cv[1], cv[2], page_table.stride(0), mask_row, pages, m, requests,
         max_draft, page_table.shape[1], words, heads, kv_heads, dim, page_size, kind, scale))
+    if requests == 0:  # the entry launches nothing: every row is one of no request
+        out.zero_()
     return out
 
 

@@ -893,6 +893,32 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   }
 }
 
+// Rows that belong to no request, before the first one's and past the last one's (what a fixed-size step carries without a
+// token), become 0: by the join, each of whose CTAs takes a share. Two loads a CTA beside its own first one where there are
+// none; where there are, the least and the largest of all starts bound them, so that in a batch whose starts are out of
+// order (0xB01) no row that some request has is touched.
+template <int kDim>
+__device__ __forceinline__ void attn_clear_outside(const AttnArgs& a, int first, int last) {
+  if (first <= 0 && last >= a.tokens) return;  // the same for the whole grid
+  __shared__ int bounds[16];
+  int lo = a.tokens, hi = 0;
+  for (int b = threadIdx.x; b <= a.requests; b += 256) {
+    const int at = min(max(a.starts[b], 0), a.tokens);
+    lo = min(lo, at), hi = max(hi, at);
+  }
+  lo = __reduce_min_sync(0xffffffffu, lo), hi = __reduce_max_sync(0xffffffffu, hi);
+  if ((threadIdx.x & 31) == 0) bounds[threadIdx.x >> 5] = lo, bounds[8 + (threadIdx.x >> 5)] = hi;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) lo = min(lo, bounds[w]), hi = max(hi, bounds[8 + w]);
+  const long long pieces = static_cast<long long>(a.heads) * (kDim / 8), all = (static_cast<long long>(lo) + a.tokens - hi) * pieces;
+  const long long step = static_cast<long long>(gridDim.x) * gridDim.y * 256;
+  for (long long i = (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < all; i += step) {
+    const long long at = i / pieces, rest = i - at * pieces, token = at < lo ? at : at - lo + hi, head = rest / (kDim / 8);
+    *reinterpret_cast<uint4*>(a.out + token * a.out_token + head * a.out_head + (rest - head * (kDim / 8)) * 8) = make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
 __host__ __device__ constexpr int attn_join_rows(int rows) { return rows >= 128 ? 8 : rows / 16; }  // rows a CTA
 
 // Joins the partials of the row tiles that cross runs: grid (runs, parts of the rows), 8 warps, of which each
@@ -908,6 +934,7 @@ __global__ void __launch_bounds__(256) tree_attn_join_kernel(const AttnArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const AttnCross x = a.cross[blockIdx.x];
+  attn_clear_outside<kDim>(a, a.starts[0], a.starts[a.requests]);
   const int r0 = blockIdx.y * kBlock;
   if (r0 >= x.rows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % kPerRow, col = r0 + warp / kPerRow;

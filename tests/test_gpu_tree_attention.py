@@ -307,3 +307,69 @@ def test_a_hidden_token_of_one_does_not_matter(drafts, hq, d, poison):
         a["k_pages"][page, :, context % 16], a["v_pages"][page, :, context % 16] = poison, poison
     got = check(a)
     assert int(torch.count_nonzero(got[0])) == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("drafts,before,after", [([1, 1], 0, 6), ([3, 0, 9], 2, 5), ([40, 33], 3, 0), ([2, 1], 1, 3000)])
+def test_rows_outside_every_request_are_zero(drafts, before, after, d):
+    """Rows before the first request's and past the last one's, as a fixed-size step's padding leaves them: zero, whatever
+    the output held, and the other rows as without them."""
+    contexts = [(1900 * b + 5) % 2500 for b in range(len(drafts))]
+    a = make(contexts, drafts, 8, 2, d, 16, torch.bfloat16, gate=True)
+    plain = check(a)
+    n = sum(drafts)
+    rows = {name: torch.full((before + n + after,) + tuple(a[name].shape[1:]), float("nan"), dtype=a[name].dtype, device="cuda") for name in ("q", "gate")}
+    for name, t in rows.items():
+        t[before:before + n] = a[name]
+    words = torch.full((before + n + after, a["tree_mask"].shape[1]), -1, dtype=torch.int32, device="cuda")
+    words[before:before + n] = a["tree_mask"]
+    b = dict(a, **rows, tree_mask=words, starts=a["starts"] + before)
+    out = torch.full((before + n + after, 3, 8, d), float("nan"), dtype=torch.bfloat16, device="cuda")
+    for to in (out[:, 1], None):
+        got = tree_attention(**b, out=to)
+        assert torch.equal(got[before:before + n], plain)
+        assert int(torch.count_nonzero(got[:before])) == 0 and int(torch.count_nonzero(got[before + n:])) == 0
+        assert device_error() == 0
+    assert torch.isnan(out[:, 0]).all() and torch.isnan(out[:, 2]).all()
+
+
+def test_rows_of_no_request_in_a_graph():
+    """A captured step of fixed size whose tokens shrink: the rows that are left over become zero."""
+    a = make([700, 20], [4, 4], 16, 2, 64, 16, torch.bfloat16)
+    out = torch.full((8, 16, 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+    tree_attention(**a, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        tree_attention(**a, out=out)
+    a["starts"].copy_(torch.tensor([0, 4, 6], dtype=torch.int32))
+    out.fill_(float("nan"))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(torch.count_nonzero(out[6:])) == 0
+    want_, bound = want(dict(a, q=a["q"][:6]))
+    assert ((out[:6].double() - want_).abs() <= bound).all()
+    a["starts"].zero_()
+    out.fill_(float("nan"))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert int(torch.count_nonzero(out)) == 0 and device_error() == 0
+
+
+def test_starts_out_of_order_keep_the_other_requests():
+    """A request whose end is before its start is reported, and rows that another one has keep their results."""
+    a = make([40, 60, 9], [5, 0, 0], 8, 2, 64, 16, torch.bfloat16)
+    plain = check(a)
+    for starts in ([0, 5, 3, 3], [0, 5, 2, 1]):
+        got = tree_attention(**dict(a, starts=torch.tensor(starts, dtype=torch.int32, device="cuda")))
+        with pytest.raises(_lib.MuseError, match="b01"):
+            device_error()
+        assert torch.equal(got, plain)
+
+
+def test_tokens_without_any_request_are_zero():
+    a = make([5], [3], 4, 1, 64, 16, torch.bfloat16, tree=None)
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    for to in (None, torch.full((3, 4, 64), float("nan"), dtype=torch.bfloat16, device="cuda")):
+        got = tree_attention(a["q"], a["k_pages"], a["v_pages"], a["page_table"][:0], none, a["starts"][:1], 1, out=to)
+        assert got.shape == (3, 4, 64) and int(torch.count_nonzero(got)) == 0 and (to is None or got is to)
+    assert device_error() == 0
