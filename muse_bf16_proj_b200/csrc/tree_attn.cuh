@@ -20,9 +20,11 @@
 // takes 8 exponentials a tile where a row-per-thread layout takes 128 on 8 lanes. dim = 64 runs the second
 // product with M = 128 on 64 dims twice over (the copy's half is not read back).
 //
-// Softmax. P is taken against a reference maximum per row that only has to be within 2^8 of the true running
-// maximum (P then stays below 256, exact enough in both 16-bit types and far from overflow in FP32 sums). A
-// tile first checks whether any score passes its reference by more than that, one barrier reduction; only then are
+// Softmax. P is taken against a reference per row that only has to be within 2^8 of the true running maximum (P then
+// stays below 256 and its sums far from overflow in FP32). FP16 holds little below 1 (halving steps end at 2^-24, and the
+// many small weights of a long context may add up to a share of the result), so its reference is set 2^7 below the
+// maximum: P stays within 2^15, weights down to 2^-31 of the largest keep a bit, and the factor cancels in the quotient. A
+// tile first checks whether any score passes its reference by more than allowed, one barrier reduction; only then are
 // the row maxima reduced across the 128 tokens, the references moved and O^T and the sums rescaled. That happens on a
 // run's first tile and rarely after. Sums of P are kept a thread (token) in FP32 and joined at the end of a run;
 // they add the rounded 16-bit values that the second product uses, so that the rounding of P cancels in the
@@ -52,7 +54,11 @@ constexpr unsigned int kErrAttnDraft = 0xB01, kErrAttnTable = 0xB02, kErrAttnPag
 constexpr unsigned int kErrAttnProducer = 0xB11, kErrAttnMma = 0xB12, kErrAttnSoftmax = 0xB13, kErrAttnDrain = 0xB14,
                        kErrAttnLoader = 0xB15;
 
-constexpr float kAttnSlack = 8.f;   // log2 of how far a score may pass its row's reference maximum
+// log2 of how far below a row's maximum its reference is set, and of how far above the reference a score may be.
+template <bool kHalf>
+constexpr float kAttnBelow = kHalf ? 7.f : 0.f;
+template <bool kHalf>
+constexpr float kAttnSlack = 8.f + kAttnBelow<kHalf>;
 constexpr int kAttnEnds = 2;        // what a row tile's beginning and end cost, in token tiles, when runs are cut
 constexpr float kAttnUnseen = -1e30f;  // reference of a row that has seen nothing: below every score, and finite
 
@@ -71,7 +77,7 @@ struct AttnArgs {
   float scale_log2;          // |scale| * log2(e)
   uint32_t q_flip;           // 0x80008000 where scale is negative: q is taken with the other sign
   struct AttnCross* cross;   // scratch: [ctas]
-  float2* part_ml;           // scratch: [ctas][2][kRows] (reference maximum, sum)
+  float2* part_ml;           // scratch: [ctas][2][kRows] (reference, sum)
   float* part_o;             // scratch: [ctas][2][kRows][dim]
 };
 
@@ -536,7 +542,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
   uint8_t* ring_v = smem + Sh::kOffV;
   uint8_t* q_s = smem + Sh::kOffQ;
   uint8_t* p_s = smem + Sh::kOffP;
-  float* ref = reinterpret_cast<float*>(smem + Sh::kOffSmall);  // reference maximum (scaled, log2)
+  float* ref = reinterpret_cast<float*>(smem + Sh::kOffSmall);  // reference (scaled, log2)
   float* rescale = ref + kRows;
   float* inv = rescale + kRows;
   int* row_ids = reinterpret_cast<int*>(inv + kRows);            // [2][kRows]: token of the request << 16 | query head
@@ -727,13 +733,13 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
               over[3] = fmaxf(over[3], fmaf(x[cc + 3], cm, -m.w));
             }
           }
-          const bool past = fmaxf(fmaxf(over[0], over[1]), fmaxf(over[2], over[3])) > kAttnSlack;
+          const bool past = fmaxf(fmaxf(over[0], over[1]), fmaxf(over[2], over[3])) > kAttnSlack<kHalf>;
           if (bar_any(8, kSoft, past || !ok)) {
             if (bar_any(8, kSoft, !ok)) {
               ok = false;
               break;
             }
-            // Move the references to the true maxima and rescale what was summed against the old ones.
+            // Move the references after the true maxima and rescale what was summed against the old ones.
 #pragma unroll
             for (int cc = 0; cc < kRows; cc += 16) {
               float top[16];
@@ -748,7 +754,7 @@ __global__ void __launch_bounds__(AttnShape<kDim, kRows>::kThreads, 1)
               const float old = ref[col];
               float now = old;
 #pragma unroll
-              for (int w = 0; w < 4 * kTG; ++w) now = fmaxf(now, red[w * kRows + col]);
+              for (int w = 0; w < 4 * kTG; ++w) now = fmaxf(now, red[w * kRows + col] - kAttnBelow<kHalf>);
               ref[col] = now;
               rescale[col] = ex2(old - now);
             }

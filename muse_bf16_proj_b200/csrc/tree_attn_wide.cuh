@@ -383,7 +383,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
           for (int k = 4; k < kN; ++k) m[k & 3] = fmaxf(m[k & 3], x[k]);
           float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * c;
           // Whether this warp (pair) or any softmax thread (lone) has a reference to move.
-          const bool past = top - ref > kAttnSlack || !ok;
+          const bool past = top - ref > kAttnSlack<kHalf> || !ok;
           if (kPair ? __any_sync(0xffffffffu, past) : bar_any(8, 256, past)) {
             if (kPair ? __any_sync(0xffffffffu, !ok) : bar_any(8, 256, !ok)) return false;
             if (!kPair) {
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(WideShape<kDim, kRows>::kThreads, 1)
               top = fmaxf(top, swap[(wg ^ 1) * 128 + tl]);
               bar_named(8, 256);
             }
-            const float now = fmaxf(ref, top), f = ex2(ref - now);
+            const float now = fmaxf(ref, top - kAttnBelow<kHalf>), f = ex2(ref - now);
             ref = now;
             l *= f;
             if (v >= step) {

@@ -373,3 +373,36 @@ def test_tokens_without_any_request_are_zero():
         got = tree_attention(a["q"], a["k_pages"], a["v_pages"], a["page_table"][:0], none, a["starts"][:1], 1, out=to)
         assert got.shape == (3, 4, 64) and int(torch.count_nonzero(got)) == 0 and (to is None or got is to)
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("draft,hq,d", [(1, 8, 64), (1, 8, 128), (6, 8, 128), (9, 8, 64), (40, 16, 128)])
+@pytest.mark.parametrize("below", [17.0, 18.5, 20.0])
+def test_fp16_weights_far_below_the_largest(draft, hq, d, below):
+    """One cached token whose score is `below` above every other one's, over a long context: the others' weights, each under
+    fp16's normal range against the largest, are a share of the result that must not be lost. (Enough requests over the
+    same pages that a CTA walks a whole context by itself.)
+
+    Bound. A weight is held against a reference at least 2^7 below fp16's range above the largest one, so its absolute
+    rounding step is 2^-25 / 2^7 of the largest weight: n steps of it times max |V| in the numerator and in the denominator.
+    Beside that the chain of attention64: p's relative rounding twice, FP32 sums, the scores, one rounding of the result."""
+    n, hk, requests, t, at = 60000, 2, 150, draft, 5
+    a = make([n], [t], hq, hk, d, 64, torch.float16, tree=None)
+    a["q"] = torch.ones((requests * t, hq, d), dtype=torch.float16, device="cuda")
+    a["page_table"] = a["page_table"].expand(requests, -1)
+    a["context"] = a["context"].expand(requests).contiguous()
+    a["starts"] = torch.arange(requests + 1, dtype=torch.int32, device="cuda") * t
+    a["k_pages"].zero_()
+    a["v_pages"].fill_(1.0)
+    page = a["page_table"][0, 0].long()
+    a["k_pages"][page, :, at] = below / math.sqrt(d)
+    a["v_pages"][page, :, at] = 0.0
+    level = a["k_pages"][page, 0, at, 0].double().item() * d * d ** -0.5  # as fp16 holds it
+    got = tree_attention(**a).double().view(requests, t, hq, d)
+    u = 2.0 ** -11
+    for i in range(t):
+        rest = (n + i) * math.exp(-level)  # the token itself and every earlier one but the largest: n + i
+        out = rest / (1.0 + rest)
+        bound = (2 * u + 2.0 ** -16 + 2 * level * 2.0 ** -18) * out + 2 * (n + i) * 2.0 ** -32
+        err = (got[:, i] - out).abs().max().item()
+        assert err <= bound + u * (out + bound), (i, err, out)
+    assert device_error() == 0
