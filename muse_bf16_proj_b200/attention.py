@@ -99,21 +99,24 @@ def page_slots(page_table: torch.Tensor, request: torch.Tensor, index: torch.Ten
 def tree_mask(parents: torch.Tensor, starts: torch.Tensor, max_draft: int) -> torch.Tensor:
     """The mask words [tokens, ceil(max_draft / 32)] int32 of drafted trees: ``parents`` [tokens] is each
     token's parent as an index among its request's drafted tokens (-1 for a root), earlier than the token
-    itself; a token sees itself and its ancestors. Made once a step, on the tensors' device."""
-    n, words = parents.shape[0], (max_draft + 31) // 32
+    itself; a token sees itself and its ancestors. What is no earlier token of the request counts as no parent, and
+    rows that belong to no request (before starts[0], from starts[B] on) see nothing. Made once a step, on the
+    tensors' device, in a few launches for each of ``max_draft`` levels."""
+    n, size = parents.shape[0], (max_draft + 31) // 32 * 32
     device = parents.device
     token = torch.arange(n, device=device)
     owner = torch.bucketize(token, starts[1:].long(), right=True)
     first = starts.long()[owner]
-    bits = torch.zeros((n, words * 32), dtype=torch.bool, device=device)
-    bits[token, token - first] = True
-    at = parents.long()
-    for _ in range(max_draft):  # one level of ancestors a turn
-        live = at >= 0
-        bits[token, at.clamp(min=0)] |= live
-        at = torch.where(live, parents.long()[(first + at.clamp(min=0)).clamp(max=max(n - 1, 0))], -1)
+    place = torch.where(owner < starts.shape[0] - 1, token - first, -1)  # among the request's tokens; negative: of none
+    up = torch.where((parents >= 0) & (parents < place), parents.long(), -1)
+    bits = torch.zeros((n, size), dtype=torch.bool, device=device)
+    at = place
+    for _ in range(max_draft):  # the token itself, then one level of ancestors a turn
+        # Every index below is inside its tensor whatever the lengths say: an indexing kernel's assertion would end the context.
+        bits[token, at.clamp(0, size - 1)] |= (at >= 0) & (at < size)
+        at = torch.where(at >= 0, up[(first + at).clamp(0, max(n - 1, 0))], -1)
     weight = 1 << torch.arange(32, device=device, dtype=torch.int64)
-    packed = (bits.view(n, words, 32).long() * weight).sum(-1)
+    packed = (bits.view(n, size // 32, 32).long() * weight).sum(-1)
     return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).int()
 
 

@@ -1,0 +1,39 @@
+"""Helpers of the operators between the projections on the CPU: the mask words of drafted trees (``tree_mask``)."""
+
+import torch
+
+from muse_bf16_proj_b200.attention import tree_mask
+
+
+def _mask_bits(words, draft):
+    return [[(int(row[j // 32]) >> (j % 32)) & 1 for j in range(draft)] for row in words.tolist()]
+
+
+def test_tree_mask_of_a_padded_step():
+    """Rows before the first request's tokens and past the last one's, any number of them, see nothing; the others what they
+    see without them."""
+    starts = torch.tensor([0, 3, 3, 8], dtype=torch.int32)
+    parents = torch.tensor([-1, 0, 0, -1, 0, 1, 1, 3], dtype=torch.int32)
+    plain = tree_mask(parents, starts, 5)
+    assert _mask_bits(plain, 5) == [[1, 0, 0, 0, 0], [1, 1, 0, 0, 0], [1, 0, 1, 0, 0], [1, 0, 0, 0, 0], [1, 1, 0, 0, 0], [1, 1, 1, 0, 0],
+                                    [1, 1, 0, 1, 0], [1, 1, 0, 1, 1]]
+    for before, after in ((0, 1), (0, 70), (40, 2)):
+        for fill in (-1, 0):
+            padded = torch.cat((torch.full((before,), fill, dtype=torch.int32), parents, torch.full((after,), fill, dtype=torch.int32)))
+            got = tree_mask(padded, starts + before, 5)
+            assert torch.equal(got[before:before + 8], plain)
+            assert int(torch.count_nonzero(got[:before])) == 0 and int(torch.count_nonzero(got[before + 8:])) == 0
+    assert tree_mask(parents[:0], torch.zeros(3, dtype=torch.int32), 5).shape == (0, 1)
+    none = tree_mask(parents, torch.zeros(1, dtype=torch.int32), 5)
+    assert none.shape == (8, 1) and int(torch.count_nonzero(none)) == 0
+
+
+def test_tree_mask_of_more_tokens_than_max_draft():
+    """What tree_attention reports as 0xB01 stays inside the words here, and the other request's rows are right."""
+    starts = torch.tensor([0, 40, 42], dtype=torch.int32)
+    parents = torch.tensor([-1] + list(range(39)) + [-1, 0], dtype=torch.int32)
+    got = tree_mask(parents, starts, 30)
+    assert got.shape == (42, 1) and _mask_bits(got[40:], 30) == [[1] + [0] * 29, [1, 1] + [0] * 28]
+    assert got[29].tolist() == [(1 << 30) - 1]
+    far = torch.tensor([500, -7, 0], dtype=torch.int32)  # no such parent
+    assert _mask_bits(tree_mask(far, torch.tensor([0, 3], dtype=torch.int32), 3), 3) == [[1, 0, 0], [0, 1, 0], [1, 0, 1]]
