@@ -91,9 +91,21 @@ def rope_table(rotary: int, positions: int, theta: float = 10000.0, scaling: str
 
 
 def page_slots(page_table: torch.Tensor, request: torch.Tensor, index: torch.Tensor, page_size: int) -> torch.Tensor:
-    """int64 slots of the tokens ``index`` (place in the request's sequence) of requests ``request``."""
-    index = index.long()
-    return page_table[request.long(), index // page_size].long() * page_size + index % page_size
+    """int64 slots of the tokens ``index`` (place in the request's sequence) of requests ``request``: -1, nothing
+    to append, where the index is negative; past every cache, which ``rope_append`` reports (0xA02) and skips, where
+    the page table has no such place (a request outside it, an index past its columns, a negative page)."""
+    request, index = request.long(), index.long()
+    requests, columns = page_table.shape
+    past = torch.iinfo(torch.int64).max
+    column = index.clamp(min=0) // page_size
+    there = (request >= 0) & (request < requests) & (column < columns)
+    if page_table.numel():
+        # Indexes are inside the table whatever the lengths say: an indexing kernel's assertion would end the context.
+        page = page_table[request.clamp(0, requests - 1), column.clamp(max=columns - 1)].long()
+        slot = torch.where(there & (page >= 0), page * page_size + index % page_size, past)
+    else:
+        slot = torch.full_like(index, past)
+    return torch.where(index < 0, -1, slot)
 
 
 def tree_mask(parents: torch.Tensor, starts: torch.Tensor, max_draft: int) -> torch.Tensor:

@@ -159,3 +159,20 @@ def test_page_slots():
     table = torch.tensor([[3, 1], [0, 2]], dtype=torch.int32, device="cuda")
     got = page_slots(table, torch.tensor([0, 0, 1], device="cuda"), torch.tensor([2, 17, 31], device="cuda"), 16)
     assert got.tolist() == [3 * 16 + 2, 16 + 1, 2 * 16 + 15]
+
+
+def test_a_token_past_its_page_table_is_reported():
+    """page_slots gives such a token a slot past every cache; the others are appended, a row without a token nowhere."""
+    q, k, v, kp, vp, _, _ = make(4, 16, 2, 64, torch.bfloat16, 16, 1)
+    table = torch.tensor([[1, -1]], dtype=torch.int32, device="cuda")
+    owner = torch.zeros(4, dtype=torch.int32, device="cuda")
+    kp.zero_()
+    for index, reported in (([0, 5, -1, 15], False), ([0, 5, 16, 15], True), ([0, 5, 32, 15], True)):
+        slots = page_slots(table, owner, torch.tensor(index, dtype=torch.int32, device="cuda"), 16)
+        rope_append(q, k, v, owner, slots, kp, vp, rope_table(64, 8))
+        if reported:
+            with pytest.raises(_lib.MuseError, match="a02"):
+                device_error()
+        else:
+            assert device_error() == 0
+        assert torch.nonzero(kp.abs().sum((1, 3)))[:, 1].tolist() == [0, 5, 15] and not kp[0].any() and not kp[2].any()

@@ -1,8 +1,9 @@
-"""Helpers of the operators between the projections on the CPU: the mask words of drafted trees (``tree_mask``)."""
+"""Helpers of the operators between the projections on the CPU: the mask words of drafted trees (``tree_mask``) and
+the slots of tokens (``page_slots``)."""
 
 import torch
 
-from muse_bf16_proj_b200.attention import tree_mask
+from muse_bf16_proj_b200.attention import page_slots, tree_mask
 
 
 def _mask_bits(words, draft):
@@ -37,3 +38,17 @@ def test_tree_mask_of_more_tokens_than_max_draft():
     assert got[29].tolist() == [(1 << 30) - 1]
     far = torch.tensor([500, -7, 0], dtype=torch.int32)  # no such parent
     assert _mask_bits(tree_mask(far, torch.tensor([0, 3], dtype=torch.int32), 3), 3) == [[1, 0, 0], [0, 1, 0], [1, 0, 1]]
+
+
+def test_page_slots_without_a_place():
+    """A row without a token (negative index) gets no slot. A place that the page table does not have (past its columns, a
+    request outside it, an entry that names no page) gets one past every cache, which rope_append reports and skips."""
+    table = torch.tensor([[3, 1], [0, -1]], dtype=torch.int32)
+    past = torch.iinfo(torch.int64).max
+    request = torch.tensor([0, 0, 1, 0, 1, 0, 1, 2, -1, 1], dtype=torch.int32)
+    index = torch.tensor([2, 17, 15, -1, -16, 32, 16, 0, 0, 1000], dtype=torch.int32)
+    assert page_slots(table, request, index, 16).tolist() == [50, 17, 15, -1, -1, past, past, past, past, past]
+    assert page_slots(table, torch.tensor([7]), torch.tensor([-1]), 16).tolist() == [-1]
+    for empty in (table[:0], table[:, :0]):
+        assert page_slots(empty, torch.tensor([0, 0]), torch.tensor([0, -1]), 16).tolist() == [past, -1]
+    assert page_slots(table, request[:0], index[:0], 16).tolist() == []
