@@ -241,13 +241,11 @@ extern "C" int muse_tree_attention(const MuseTreeAttention* p, void* stream) {
   muse::AttnArgs a;
   a.q = static_cast<const uint16_t*>(p->q);
   a.gate = static_cast<const uint16_t*>(p->gate);
-  a.k_pages = static_cast<const uint16_t*>(p->k_pages);
   a.v_pages = static_cast<const uint16_t*>(p->v_pages);
   a.out = static_cast<uint16_t*>(p->out);
   a.table = p->table, a.context = p->context, a.starts = p->starts, a.mask = p->mask;
   a.q_token = p->q_token, a.q_head = p->q_head, a.gate_token = p->gate_token, a.gate_head = p->gate_head;
   a.out_token = p->out_token, a.out_head = p->out_head;
-  a.k_page = p->k_page, a.k_head = p->k_page_head, a.k_slot = p->k_entry;
   a.v_page = p->v_page, a.v_head = p->v_page_head, a.v_slot = p->v_entry;
   a.table_row = p->table_row, a.mask_row = p->mask_row, a.pages = p->pages;
   a.requests = p->requests, a.tokens = p->tokens, a.max_draft = p->max_draft, a.table_cols = p->table_cols;

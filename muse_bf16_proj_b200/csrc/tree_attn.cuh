@@ -63,12 +63,12 @@ constexpr int kAttnEnds = 2;        // what a row tile's beginning and end cost,
 constexpr float kAttnUnseen = -1e30f;  // reference of a row that has seen nothing: below every score, and finite
 
 struct AttnArgs {
-  const uint16_t *q, *gate, *k_pages, *v_pages;
+  const uint16_t *q, *gate, *v_pages;  // K is reached through its tensor map alone
   uint16_t* out;
   const int32_t *table, *context, *starts;
   const uint32_t* mask;
   long long q_token, q_head, gate_token, gate_head, out_token, out_head;
-  long long k_page, k_head, k_slot, v_page, v_head, v_slot;
+  long long v_page, v_head, v_slot;
   long long table_row, mask_row;
   long long pages;
   int requests, tokens, max_draft, table_cols, heads, kv_heads, page;
