@@ -406,3 +406,17 @@ def test_fp16_weights_far_below_the_largest(draft, hq, d, below):
         err = (got[:, i] - out).abs().max().item()
         assert err <= bound + u * (out + bound), (i, err, out)
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("prompt,context,hq,hk,d", [(600, 100, 8, 2, 64), (513, 0, 4, 1, 128)])
+def test_a_prompt_in_pieces(prompt, context, hq, hk, d):
+    """A prompt of more than 256 tokens as requests of up to 256 over the same pages, each after the ones before it, against
+    the prompt as one request of the 64-bit form."""
+    a = make([context], [prompt], hq, hk, d, 16, torch.bfloat16, tree=None, gate=True)
+    out, bound = want(a)
+    starts = list(range(0, prompt, 256)) + [prompt]
+    pieces = len(starts) - 1
+    got = tree_attention(a["q"], a["k_pages"], a["v_pages"], a["page_table"].expand(pieces, -1),
+                         torch.tensor([context + s for s in starts[:-1]], dtype=torch.int32, device="cuda"),
+                         torch.tensor(starts, dtype=torch.int32, device="cuda"), 256, gate=a["gate"])
+    assert ((got.double() - out).abs() <= bound).all() and device_error() == 0

@@ -11,6 +11,7 @@ import torch
 from muse_bf16_proj_b200 import _lib
 from muse_bf16_proj_b200.attention import rope_table
 from muse_bf16_proj_b200.contract import generate_weights
+from muse_bf16_proj_b200.routing import route
 from muse_bf16_proj_b200.submission import prepare, project
 from muse_bf16_proj_b200.verify_step import DIM, HEADS, KV_HEADS, make_batch, random_trees, verify_step
 from serving_ref import attention64, rope64, route64
@@ -73,3 +74,26 @@ def test_step_as_a_graph(model):
     torch.cuda.synchronize()
     for name, t in eager.items():
         assert torch.equal(t, captured[name]), name
+
+
+def test_other_experts_are_near_ties(model):
+    """Where the step's choice differs from the 64-bit one of its own logits, the experts (or groups) that changed places are
+    worth the same to within 32-bit rounding. A score up to 1 is off by at most 2^-22 (exp 2^-23, its sum with 1 and the
+    quotient 2^-24 each), score + bias by 2^-24 more, and two of them are compared: under 2^-20. A group's worth adds two
+    with one rounding more: under 2^-19."""
+    _, state = model
+    g = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn((700, 8192), generator=g, device="cuda").bfloat16()
+    balance = 0.05 * torch.randn(256, generator=g, device="cuda")
+    logits = project(x, state, "router")
+    _, experts = route(logits, 8, scoring="sigmoid", bias=balance, groups=8, top_groups=4)
+    _, exact = route64(logits, 8, "sigmoid", balance, 8, 4, True, 1.0)
+    choice = torch.sigmoid(logits.double().cpu()) + balance.double().cpu()
+    worth = choice.view(-1, 8, 32).topk(2, dim=-1)[0].sum(-1)
+    for t in torch.nonzero((experts.cpu() != exact).any(1))[:, 0].tolist():
+        kept = worth[t].topk(4)
+        limit, groups = kept[0][-1].item(), set((experts[t].cpu() // 32).tolist())
+        assert all(worth[t, group].item() >= limit - 2.0 ** -19 for group in groups), t
+        if groups <= set(kept[1].tolist()) and set((exact[t] // 32).tolist()) <= set(kept[1].tolist()):
+            mine, other = choice[t][experts[t].cpu().long()], choice[t][exact[t].long()]
+            assert ((mine - other).abs() <= 2.0 ** -20).all(), t

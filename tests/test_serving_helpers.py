@@ -1,9 +1,11 @@
-"""Helpers of the operators between the projections on the CPU: the mask words of drafted trees (``tree_mask``) and
-the slots of tokens (``page_slots``)."""
+"""Helpers of the operators between the projections on the CPU: the mask words of drafted trees (``tree_mask``),
+the slots of tokens (``page_slots``) and the ramp of a stretched rotary table (``rope_table``)."""
+
+import math
 
 import torch
 
-from muse_bf16_proj_b200.attention import page_slots, tree_mask
+from muse_bf16_proj_b200.attention import page_slots, rope_table, tree_mask
 
 
 def _mask_bits(words, draft):
@@ -52,3 +54,25 @@ def test_page_slots_without_a_place():
     for empty in (table[:0], table[:, :0]):
         assert page_slots(empty, torch.tensor([0, 0]), torch.tensor([0, -1]), 16).tolist() == [past, -1]
     assert page_slots(table, request[:0], index[:0], 16).tolist() == []
+
+
+def test_yarn_blends_by_the_pairs_index():
+    """Every entry of the ramp: the share of the divided frequency rises linearly from the pair that turns beta_fast times in
+    the original positions to the one that turns beta_slow times."""
+    rot, theta, original, f = 64, 10000.0, 8192, 4.0
+    table = rope_table(rot, 4000, theta, "yarn", f, original, device="cpu")
+    freq = [theta ** (-2 * i / rot) for i in range(rot // 2)]
+
+    def turns(i):
+        return original * freq[i] / (2 * math.pi)
+
+    # The last pair that turns at least 32 times, the first that turns at most once.
+    first = max(i for i in range(rot // 2) if turns(i) >= 32)
+    last = min(i for i in range(rot // 2) if turns(i) <= 1)
+    assert 0 < first < last - 1 < rot // 2 - 2  # a ramp with entries inside
+    magnitude = 0.1 * math.log(f) + 1.0
+    for i in range(rot // 2):
+        share = min(max((i - first) / (last - first), 0.0), 1.0)
+        angle = 3999 * (freq[i] / f * share + freq[i] * (1 - share))
+        for got, exact in ((table[3999, i], math.cos(angle)), (table[3999, rot // 2 + i], math.sin(angle))):
+            assert abs(got.item() - magnitude * exact) < 1e-6, (i, share)
