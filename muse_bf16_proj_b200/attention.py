@@ -28,7 +28,7 @@ import torch
 from . import _lib
 
 _TYPES = {torch.bfloat16: _lib.TYPE_BF16, torch.float16: _lib.TYPE_F16}
-MAX_DRAFT = 256  # drafted tokens of one request
+MAX_DRAFT = 256  # drafted tokens of one request; longer prompts go in pieces over the same pages
 
 
 def split_qkv_gate(y: torch.Tensor, heads: int, kv_heads: int, dim: int):
@@ -119,14 +119,16 @@ def tree_mask(parents: torch.Tensor, starts: torch.Tensor, max_draft: int) -> to
     token = torch.arange(n, device=device)
     owner = torch.bucketize(token, starts[1:].long(), right=True)
     first = starts.long()[owner]
-    place = torch.where(owner < starts.shape[0] - 1, token - first, -1)  # among the request's tokens; negative: of none
+    place = token - first  # among the request's tokens
+    place = torch.where((owner < starts.shape[0] - 1) & (place < size), place, -1)  # negative: of none, or without a bit
     up = torch.where((parents >= 0) & (parents < place), parents.long(), -1)
     bits = torch.zeros((n, size), dtype=torch.bool, device=device)
     at = place
     for _ in range(max_draft):  # the token itself, then one level of ancestors a turn
         # Every index below is inside its tensor whatever the lengths say: an indexing kernel's assertion would end the context.
-        bits[token, at.clamp(0, size - 1)] |= (at >= 0) & (at < size)
-        at = torch.where(at >= 0, up[(first + at).clamp(0, max(n - 1, 0))], -1)
+        live = at >= 0
+        bits[token, at.clamp(min=0)] |= live
+        at = torch.where(live, up[(first + at).clamp(0, max(n - 1, 0))], -1)
     weight = 1 << torch.arange(32, device=device, dtype=torch.int64)
     packed = (bits.view(n, size // 32, 32).long() * weight).sum(-1)
     return torch.where(packed >= 1 << 31, packed - (1 << 32), packed).int()
