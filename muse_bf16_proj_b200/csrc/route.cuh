@@ -72,6 +72,12 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+// A group's worth by its best two choices. An infinite best one is the worth itself: with a bias of +inf and the rest of the
+// group masked the sum would be NaN, which no rank counts, and a group more than top_groups would stay.
+__device__ __forceinline__ float group_worth(float best, float second) {
+  return fabsf(best) == __int_as_float(0x7f800000) ? best : best + second;
+}
+
 // kJ: 128-expert blocks (count <= 128 * kJ).
 template <int kType, int kJ>
 __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs a) {
@@ -170,7 +176,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
         b2 = max(max(b2, d2), min(b1, d1));
         b1 = max(b1, d1);
       }
-      worth[j] = a.bias ? key_value(b1) + key_value(b2) : key_value(b1);
+      worth[j] = a.bias ? group_worth(key_value(b1), key_value(b2)) : key_value(b1);
     }
     // Rank of each held group: groups of a block follow one another over its lanes.
     const int in_block = 32 / a.group_lanes, mine = lane / a.group_lanes;
@@ -219,7 +225,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) route_kernel(const RouteArgs
       b2 = fmaxf(fmaxf(b2, c2), fminf(b1, c1));
       b1 = fmaxf(b1, c1);
     }
-    const float worth = a.bias ? (a.group_size > 1 ? b1 + b2 : b1) : b1;
+    const float worth = a.bias && a.group_size > 1 ? group_worth(b1, b2) : b1;
     int rank = 0;
     for (int o = 0; o < a.groups; ++o) {
       const float w = __shfl_sync(0xffffffffu, worth, o * per);

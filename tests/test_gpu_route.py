@@ -151,3 +151,29 @@ def test_bias_written_just_before():
         want = route64(logits, 8, "sigmoid", offsets.clone(), 8, 4, True, 1.0)[1]
         graph.replay()
         assert torch.equal(e.cpu(), want)
+
+
+@pytest.mark.parametrize("experts", [32, 24])
+def test_an_infinite_bias_in_a_masked_group(experts):
+    """An expert with a bias of +inf whose group is masked but for it: the group is worth +inf (not inf - inf), and no more than
+    ``top_groups`` groups take part."""
+    size = experts // 4
+    g = torch.Generator(device="cuda").manual_seed(experts)
+    logits = torch.randn((50, experts), generator=g, device="cuda")
+    logits[:, 2 * size:3 * size] = -float("inf")
+    forced = 2 * size + 3
+    logits[:, forced] = 0.25
+    bias = 0.05 * torch.randn(experts, generator=g, device="cuda")
+    bias[forced] = float("inf")
+    top_k = size + 1
+    weights, chosen = route(logits, top_k, scoring="sigmoid", bias=bias, groups=4, top_groups=2, renormalize=False)
+    scores = torch.sigmoid(logits.double())
+    choice = (scores + bias.double()).cpu()
+    worth = choice.view(50, 4, size).topk(2, dim=-1)[0].sum(-1)
+    worth[:, 2] = -float("inf")  # the other of the two groups
+    best = worth.argmax(1)
+    for t in range(50):
+        order = choice[t, best[t] * size:(best[t] + 1) * size].argsort(descending=True) + best[t] * size
+        assert chosen[t].tolist() == [forced] + order.tolist()
+    assert ((weights.double() - torch.gather(scores, 1, chosen.long())).abs() <= 2.0 ** -22).all()
+    assert _lib.device_error(torch.cuda.current_stream().cuda_stream) == 0
