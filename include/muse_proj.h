@@ -529,7 +529,7 @@ int muse_tree_attention_scratch_bytes(const MuseTreeAttention* args, int64_t* by
 /*
  * The top_k experts of each token and their weights. Scores: softmax over the experts, or sigmoid. Choice: the
  * logits without a bias, score + bias with one (the bias never enters a weight). groups > 1: experts
- * g * experts / groups .. are group g, worth its best choice (with a bias: its best two added); only the best
+ * g * experts / groups .. are group g, worth its best choice (with a bias: its best two added, an infinite best one alone); only the best
  * top_groups groups stay. Chosen in descending order, ties to the lowest index. weights = the chosen scores, divided
  * by their sum if renormalize (0 where that is 0), times scale. A NaN logit counts as -inf; an expert of -inf is
  * chosen after every other and weighs 0.

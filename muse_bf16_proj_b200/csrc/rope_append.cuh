@@ -8,9 +8,10 @@
 // Bound: bytes (q, k, v in; q and the cache rows out), 16-byte accesses throughout. A thread owns one
 // 16-element piece of a head (eight pairs) and walks heads with it, so its table entries are loaded
 // once a token and stay in registers; a CTA covers 8 (dim 128) or 16 (dim 64) heads at a time.
-// Rotary sizes, strides or pointers that rule out 16-byte accesses take the scalar kernel, one pair a
-// thread. Measured: 4096 tokens of 64 + 2 x 8 heads of 128 (170 MB) in 29.4 us = 5.8 TB/s, 0.88 of a plain
-// copy's rate; 201 tokens in 3.5 us and one in 2.7 us, which is the launch.
+// Rotary sizes that are no multiple of 16, strides or pointers that rule out 16-byte accesses take the scalar kernel
+// for the whole row, one pair a thread. Measured, device time: 4096 tokens of 64 + 2 x 8 heads of 128 (170 MB) in 29.0 us =
+// 5.85 TB/s, 0.89 of a plain copy's rate, at rotary 128 and 64 and for both kinds of pairs; in 111 us by the scalar kernel
+// (rotary 36 and 20); 201 tokens in 3.0 us and one in 2.3 us, which is the launch.
 #pragma once
 
 #include <cuda_bf16.h>

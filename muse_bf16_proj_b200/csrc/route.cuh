@@ -14,8 +14,9 @@
 // the issue of its instructions (66 % of all slots at 8192 tokens); the bytes (4 a logit, 8.9 MB and 1.4 us there)
 // are far below it.
 //
-// Scores are computed with expf and IEEE division, each operation rounded once, so that score + bias has
-// the bits of the same elementary operations anywhere else, and near ties fall the same way. NaN logits
+// Scores are computed with expf and IEEE division, each operation rounded once, so that a sigmoid's score + bias has
+// the bits of the same elementary operations anywhere else, and near ties fall the same way; with softmax the sum over the
+// experts is added in the warp's own order, and near ties under a bias may fall otherwise. NaN logits
 // count as -inf; an expert of -inf is chosen after every other, lowest index first, and weighs 0. A token
 // whose chosen scores sum to 0 has weights 0.
 #pragma once

@@ -105,8 +105,10 @@ int check_attention(const MuseTreeAttention* p) {
 // Rows of a unit: those that share a kv head, rounded up to a variant. Tokens-as-M up to 32 rows, rows-as-M past that.
 // Measured, tokens-as-M and rows-as-M, at 1 x 700, 1 x 20000, 8 x 3000 and 16 x 20000 (requests x entries), 8 kv heads of
 // 128: 20 rows 12.1 and 12.6, 22.1 and 25.2, 20.8 and 21.0, 132 and 132 us; 64 rows (a softmax thread a token and 32
-// columns) 14.9 and 13.4, 27.5 and 26.4, 26.9 and 24.4, 142 and 133 us. 2 kv heads of 64: 32 rows 11.9 and 9.7, 14.8 and
-// 20.5, 14.1 and 13.3, 28.9 and 37.2 us.
+// columns; that variant is gone) 14.9 and 13.4, 27.5 and 26.4, 26.9 and 24.4, 142 and 133 us. 2 kv heads of 64, these four
+// and 32 x 4096 and 64 x 1000: 20 rows 10.9 and 9.5, 14.1 and 20.0, 13.1 and 13.0, 27.6 and 37.1, 20.0 and 22.0, 19.2 and
+// 18.6 us; 32 rows 11.7 and 9.7, 14.7 and 20.2, 13.9 and 13.3, 28.5 and 37.3, 20.8 and 22.0, 20.0 and 18.7 us. There neither
+// side wins throughout: tokens-as-M gives up 2 us at most and gains up to 9, and the lengths that decide are the device's.
 int attention_rows(const MuseTreeAttention* p) {
   const int64_t rows = static_cast<int64_t>(p->max_draft) * (p->heads / p->kv_heads);
   return rows <= 16 ? 16 : (rows <= 32 ? 32 : (rows <= 128 ? 128 : 256));

@@ -5,10 +5,10 @@
 //
 // Bound: the cache is read once (4 * dim bytes a token and kv head), so up to a few dozen rows a kv head the kernel
 // is a stream of K and V tiles from HBM; the matrix products only have to keep up. Measured with the join, 8 kv heads of
-// 128, bf16: 537 MB of cache (one token of 64 heads over 131072 entries) in 84.2 us = 6.38 TB/s, 0.97 of a plain copy's
-// rate; 336 MB (32 requests of 1024 to 4096 entries, pages of 16) in 58.5 us = 5.75 TB/s, 0.88: about 3 us pass before
-// the first tile and 3 us in the join. Short calls are latency: 700 entries of 2 heads of 64 take 9.5 us, of which the
-// cut of the runs is 1 us, the first Q and K 2 us and the join 2.4 us.
+// 128, bf16, device time of a call: 537 MB of cache (one token of 64 heads over 131072 entries) in 83.6 us = 6.42 TB/s, 0.98
+// of a plain copy's rate; 336 MB (32 requests of 1024 to 4096 entries, pages of 16) in 58.1 us = 5.78 TB/s, 0.88: about 3 us
+// pass before the first tile and 3 us in the join. Short calls are latency: 700 entries of 2 heads of 64 take 9.1 us, of
+// which the cut of the runs is 1 us, the first Q and K 2 us and the join 2.4 us.
 //
 // Shape. The rows of a request that share a kv head (tokens x heads / kv_heads) are one operand, cut into row tiles of
 // kRows (16 or 32; more rows take the rows-as-M kernel of tree_attn_wide.cuh). Tokens are the tensor cores'
@@ -26,9 +26,12 @@
 // maximum: P stays within 2^15, weights down to 2^-31 of the largest keep a bit, and the factor cancels in the quotient. A
 // tile first checks whether any score passes its reference by more than allowed, one barrier reduction; only then are
 // the row maxima reduced across the 128 tokens, the references moved and O^T and the sums rescaled. That happens on a
-// run's first tile and rarely after. Sums of P are kept a thread (token) in FP32 and joined at the end of a run;
-// they add the rounded 16-bit values that the second product uses, so that the rounding of P cancels in the
-// quotient of rows that one token dominates.
+// run's first tile and rarely after. P is rounded to the cache's type because the second product's operands have one
+// type, which is V's; its weights are then off by up to 2^-9 (BF16) or 2^-12 (FP16) each, and results are 1.1 to 1.4 times
+// as far from the exact ones as with P in FP32 (one token over 131072 entries 2.3e-3 against 1.7e-3, of which the output's
+// own rounding is 1.7e-3). Sums of P are kept a thread (token) in FP32 and joined at the end of a run; they add the rounded
+// values that the second product uses, so that the rounding of P cancels in the quotient of rows that one token dominates.
+// ex2.approx (about 2^-22) and, in the gate, __expf and __fdividef (under 2^-18 up to |gate| = 20) are far below either.
 //
 // Split. One CTA an SM; all (request, row tile, kv head, token tile) units in that order are cut into equal
 // contiguous runs, one a CTA, from lengths read on the device (no host synchronisation, graph-safe). A row tile

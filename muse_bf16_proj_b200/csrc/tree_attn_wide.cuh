@@ -5,12 +5,14 @@
 //   S [128 rows x 128 tokens] = Q . K^T            (both K-major from shared memory)
 //   O [128 rows x dim]       += P . V              (P from tensor memory over S's columns, V as stored, N-major)
 // A row is a TMEM lane and one softmax thread's, so its maximum, its references and its sums need no other thread,
-// and P never passes through shared memory. Bound: at 2 x 128 rows the two products take 1024 tensor cycles a tile at
-// dim 128 and its 16384 exponentials as many cycles of the exponential unit; K and V come in once for both. Measured: 16
-// requests of 64 tokens, 64 heads over 8 of 128, up to 8192 entries (174 GFLOP) in 205 us with the join = 850 TFLOP/s,
-// 0.51 of a dense product's rate, the tensor cores busy 44 % of the cycles and no other unit above that: one S at a time
-// passes from the products to a softmax and back, and each of those hand-offs is on the chain (TMEM has no room for a
-// second S at dim 128). 33 to 128 rows over 822 MB of cache take 132 to 141 us = 6.2 to 5.8 TB/s; 52 rows over 84 MB
+// and P never passes through shared memory. Bound: at 2 x 128 rows the two products of both take 2048 tensor cycles a tile at
+// dim 128 and the 32768 exponentials as many cycles of the exponential unit, so the two bind alike; K and V come in once for
+// both row tiles. Measured: 16 requests of 64 tokens, 64 heads over 8 of 128, up to 8192 entries (174 GFLOP) in 205 us with
+// the join in short runs = 850 TFLOP/s, 0.51 of a dense product's rate; in calls one after another 244 to 255 us = 710 to
+// 680 TFLOP/s, where the power limit holds the SM clock near 1630 of 1965 MHz (241 us a call from a graph at that clock). The
+// tensor cores are busy 44 % of the cycles: one S at a time passes from the products to a softmax and back, and each of those
+// hand-offs is on the chain (TMEM has no room for a second S at dim 128). A softmax thread of the 256-row variants holds 128
+// scores under the 168 registers that 384 threads leave it and spills 132 or 136 bytes (the 128-row ones none). 33 to 128 rows over 822 MB of cache take 132 to 141 us = 6.2 to 5.8 TB/s; 52 rows over 84 MB
 // (11 requests of up to 13 tokens) take 25 us against 12.7 of bytes: the start, the row tiles' ends and the join.
 //
 // Two row tiles alternate ("pair"): while one's softmax runs, the tensor cores do the other's products. Each has its
